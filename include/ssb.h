@@ -61,13 +61,19 @@ typedef struct SsbSplats {
 } SsbSplats;
 
 /* Quantised SH value storage, QuantizedTensor<BITS,256> (src/core/Tensor.h:1313-1404)
- * as read by the projection kernels (src/shaders/harmonics.slang:115-140). */
+ * as read by the projection kernels (src/shaders/harmonics.slang:115-140).
+ * bits = 4 has no counterpart in the reference: one 32-byte row per splat, on a 32-byte boundary, holding the 45 values as
+ * four-bit codes with one scale per SH band.  As little-endian 32-bit words: words 2c and 2c + 1 are channel c, coefficient
+ * j's value being scale * (((word[2c + j / 8] >> 4 (j % 8)) & 15) - 8), the code 0 not being written; words 6 and 7 hold the
+ * scales as bf16 bits, band 1 in the low and band 2 in the high half of word 6, band 3 in the low half of word 7.  An all-zero
+ * row stands for zeros.  Read by every call that takes an SsbShQuant; written by ssb_quant_encode.  The optimiser does not update
+ * it: a trainer keeps fp32 values, encodes them before an iteration's views and applies the gradients to the fp32 values. */
 typedef struct SsbShQuant {
-    void* packed;          /* uint8 [n*45] or uint16 [n*45]; NULL = fp32 SH */
-    float* bounds;         /* float2 (min,max) per block of `bounds_stride` cells */
-    int32_t bits;          /* 8 or 16 (32 / 0 = not quantised) */
+    void* packed;          /* uint8 [n*45] or uint16 [n*45], or 32-byte rows [n]; NULL = fp32 SH */
+    float* bounds;         /* float2 (min,max) per block of `bounds_stride` cells (not read when bits = 4) */
+    int32_t bits;          /* 4, 8 or 16 (32 / 0 = not quantised) */
     int32_t reserved;
-    int64_t bounds_stride; /* cells per bound; 256 for the per-cell-block layout */
+    int64_t bounds_stride; /* cells per bound; 256 for the per-cell-block layout (not read when bits = 4) */
 } SsbShQuant;
 
 /* One batch of cameras sharing size and model.
@@ -168,6 +174,55 @@ int ssb_project_bwd(const SsbSplats* splats, const SsbShQuant* shq, int64_t n,
                     const SsbCameras* cams, const float* d_aabb,
                     const SsbScreenRec* d_v_screen,
                     const SsbSplats* grads, int accumulate, void* stream);
+
+/* ---- spherical harmonics on their own ----------------------------------- */
+
+/* The value of every splat's spherical harmonics in the direction of every view, for callers that project by other means or
+ * bake colours (inside the projection calls above the same product is part of the projection):
+ *   d_values[v][i][ch] = 0.28209479 features_dc[i][ch] + sum_j b_j(dir) SH[i][j][ch],   [cams->count][n][3] floats,
+ * dir = the unit vector from the camera centre of view v to means[i], b_1.. the real basis of
+ * src/shaders/harmonics.slang:154-251.  The colour of the projection is max(value + 0.5, 0).
+ * Of `splats`, means, features_dc (NULL: zeros) and features_sh (when shq names no codes) are read; of `cams`, d_viewmats,
+ * count and sh_degree_plus1.  A splat at the camera's centre has no direction: its value is the features_dc term.
+ * ssb_sh_eval_bwd: gradients of means, features_dc and features_sh (the coefficients' values, whatever they are stored in), summed
+ * over the views in view order; an array that is NULL in `grads` is not wanted.  accumulate != 0 adds to the arrays.  Coefficients
+ * above the active degree get zero. */
+int ssb_sh_eval_fwd(const SsbSplats* splats, const SsbShQuant* shq, int64_t n, const SsbCameras* cams, float* d_values, void* stream);
+int ssb_sh_eval_bwd(const SsbSplats* splats, const SsbShQuant* shq, int64_t n, const SsbCameras* cams, const float* d_v_values,
+                    const SsbSplats* grads, int accumulate, void* stream);
+
+/* ---- dropout ------------------------------------------------------------- */
+
+/* Dropout of splat parameters, the regulariser of captures with few views: what an iteration's views read is a copy of an
+ * array in which groups of values are set to zero at random and the rest is scaled by 1 / (1 - rate).  No counterpart in the
+ * reference.  The decision for group g is word g % 4 of Philox4x32-10 with counter (g / 4, offset) and key `seed`, two 32-bit
+ * words each, low word first: dropped when the word is below floor(rate * 2^32).  No mask is stored: the backward call, with
+ * the same description, makes the same one.  Give each iteration its own offset and each array its own seed. */
+typedef struct SsbDropout {
+    float rate;                  /* in [0, 1) */
+    int32_t reserved;            /* 0 */
+    uint64_t seed;
+    uint64_t offset;
+    const uint64_t* d_offset;    /* device word added to `offset` when the kernel runs, or NULL: a captured graph draws a new mask
+                                  * on every replay when the word is advanced in between */
+} SsbDropout;
+enum { SSB_DROPPED_LOGIT = -64 };
+
+/* d_y[k] = 0 or d_x[k] / (1 - rate) for `count` values, `group` consecutive values of the whole array sharing one decision
+ * (SH array: 1 = every value, 3 = a coefficient's three colours, 45 = a splat's row).  `first` is the number in the whole array
+ * of the value that d_x and d_y point at, so a shard draws what the whole would.  Values in dropped places are not looked at (NaN
+ * and infinities become zero).  d_y may be d_x.  The operator is linear: its backward is the same call on the gradients. */
+int ssb_dropout(const float* d_x, int64_t first, int64_t count, int32_t group, const SsbDropout* dropout, float* d_y, void* stream);
+
+/* Dropout of whole splats through their opacities, logits to logits: a kept splat's opacity becomes
+ * min(sigmoid(x) / (1 - rate), 0.999) (the rasteriser's own limit on alpha), a dropped one's logit SSB_DROPPED_LOGIT, far below
+ * what the projection keeps, so that it is culled in every view and receives no gradient.  Splat k of the arrays is splat
+ * first + k of the model; one decision per splat.  rate = 0 copies.  d_out may be d_opacities.
+ * The backward call takes d(loss)/d(d_out) and gives d(loss)/d(d_opacities): zero where the splat was dropped or its opacity
+ * limited.  d_opacities are the stored logits; d_v_opacities may be d_v_out. */
+int ssb_dropout_opacities(const float* d_opacities, int64_t first, int64_t count, const SsbDropout* dropout, float* d_out, void* stream);
+int ssb_dropout_opacities_bwd(const float* d_opacities, const float* d_v_out, int64_t first, int64_t count, const SsbDropout* dropout,
+                              float* d_v_opacities, void* stream);
 
 /* Record <-> reference ScreenBuffer arrays (xy [m][2], depth [m], conic [m][3],
  * opac [m], rgb [m][3]); src/primitives/PrimitiveBase3DGS.cuh:187-211. */
@@ -507,7 +562,11 @@ int ssb_adam_step_sh_quantized_ex(float* d_grad, uint8_t* d_optim_packed, float*
                                   const SsbAdamConfig* cfg, const int32_t* d_steps, int32_t cells_per_splat, void* stream);
 
 /* QuantizedTensor<BITS,256>::encode_v / decode_v over whole buffers
- * (src/core/Tensor.h:1366-1393); bounds = float2 per 256 cells. */
+ * (src/core/Tensor.h:1366-1393); bounds = float2 per 256 cells.
+ * bits = 4: the 32-byte rows of SsbShQuant, numel = 45 * splats, d_bounds is not used (NULL).  A band's scale is the smallest bf16
+ * number s with 7 s >= m, m the largest finite magnitude of the band (0 when m < 2^-100; one step
+ * smaller where 7 s would overflow), and a value's code is value / s rounded
+ * to the nearest integer, ties to even, at most 7 in magnitude: NaN becomes 0 and an infinity +-7.  Decoding is exact. */
 int ssb_quant_encode(const float* d_values, int64_t numel, int32_t bits, void* d_packed, float* d_bounds, void* stream);
 int ssb_quant_decode(const void* d_packed, const float* d_bounds, int64_t numel, int32_t bits, float* d_values, void* stream);
 

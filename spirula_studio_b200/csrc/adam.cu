@@ -1221,8 +1221,14 @@ int ssb_exchange_step_q16(const SsbPeerReplicas* replicas, const SsbSplats* para
 
 int ssb_quant_encode(const float* d_values, int64_t numel, int32_t bits, void* d_packed, float* d_bounds, void* stream) {
     using namespace ssb;
+    if (bits == 4) {
+        SSB_REQUIRE(((d_values && d_packed) || numel == 0) && numel >= 0 && numel % (3 * kNumSh) == 0, "ssb_quant_encode: 4-bit rows take whole splats of 45 values");
+        SSB_REQUIRE(((uintptr_t)d_packed & 31) == 0 && ((uintptr_t)d_values & 3) == 0,
+                    "ssb_quant_encode: 4-bit SH rows must start on a 32-byte boundary, values on a 4-byte one");
+        return launch_sh_rows_encode(d_values, numel / (3 * kNumSh), d_packed, (cudaStream_t)stream);
+    }
     SSB_REQUIRE(d_values && d_packed && d_bounds && numel >= 0, "ssb_quant_encode: bad argument");
-    SSB_REQUIRE(bits == 8 || bits == 16, "ssb_quant_encode: bits must be 8 or 16 (got %d)", bits);
+    SSB_REQUIRE(bits == 8 || bits == 16, "ssb_quant_encode: bits must be 4, 8 or 16 (got %d)", bits);
     if (numel == 0) return SSB_OK;
     unsigned blocks = (unsigned)ceil_div(numel, 256);
     if (bits == 8) quant_encode_kernel<8><<<blocks, 256, 0, (cudaStream_t)stream>>>(d_values, numel, (uint8_t*)d_packed, (float2*)d_bounds);
@@ -1233,8 +1239,14 @@ int ssb_quant_encode(const float* d_values, int64_t numel, int32_t bits, void* d
 
 int ssb_quant_decode(const void* d_packed, const float* d_bounds, int64_t numel, int32_t bits, float* d_values, void* stream) {
     using namespace ssb;
+    if (bits == 4) {
+        SSB_REQUIRE(((d_values && d_packed) || numel == 0) && numel >= 0 && numel % (3 * kNumSh) == 0, "ssb_quant_decode: 4-bit rows hold whole splats of 45 values");
+        SSB_REQUIRE(((uintptr_t)d_packed & 31) == 0 && ((uintptr_t)d_values & 3) == 0,
+                    "ssb_quant_decode: 4-bit SH rows must start on a 32-byte boundary, values on a 4-byte one");
+        return launch_sh_rows_decode(d_packed, numel / (3 * kNumSh), d_values, (cudaStream_t)stream);
+    }
     SSB_REQUIRE(d_values && d_packed && d_bounds && numel >= 0, "ssb_quant_decode: bad argument");
-    SSB_REQUIRE(bits == 8 || bits == 16, "ssb_quant_decode: bits must be 8 or 16 (got %d)", bits);
+    SSB_REQUIRE(bits == 8 || bits == 16, "ssb_quant_decode: bits must be 4, 8 or 16 (got %d)", bits);
     if (numel == 0) return SSB_OK;
     unsigned blocks = (unsigned)ceil_div(numel, 256);
     if (bits == 8) quant_decode_kernel<8><<<blocks, 256, 0, (cudaStream_t)stream>>>((const uint8_t*)d_packed, (const float2*)d_bounds, numel, d_values);

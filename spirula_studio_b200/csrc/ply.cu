@@ -16,7 +16,7 @@
 // The reader follows the reference's (src/checkpoint/SplatPly.cpp:65-254): any order and any scalar type of the vertex
 // properties, binary little endian or ASCII, other elements ignored, a list property on the vertex element refused; it
 // needs x y z, opacity, scale_*, rot_*, f_dc_*; f_rest_* give the SH degree (0 when absent) and are transposed back.
-#include "ssb_common.cuh"
+#include "sh_device.cuh"
 
 #include <algorithm>
 #include <cctype>
@@ -37,6 +37,12 @@ constexpr float kPlyOpacityMin = -5.5373f;                            // logit(1
 __device__ __forceinline__ float ply_sh_value(const SsbSplats& p, const SsbShQuant& q, int64_t splat, int j, int ch) {
     const int64_t cell = splat * (3 * kNumSh) + 3 * j + ch;
     if (q.packed == nullptr) return p.features_sh[cell];
+    if (q.bits == 4) {
+        const uint32_t* w = (const uint32_t*)((const char*)q.packed + kShRowBytes * splat);
+        const int code = (int)((w[2 * ch + (j >> 3)] >> (4 * (j & 7))) & 15u) - 8;
+        const int band = sh_band(j);
+        return __uint_as_float(band == 1 ? w[6] & 0xffff0000u : (band == 0 ? w[6] : w[7]) << 16) * (float)code;
+    }
     const int64_t b = cell / q.bounds_stride;
     const float lo = q.bounds[2 * b], hi = q.bounds[2 * b + 1];
     if (q.bits == 8) return lo + (hi - lo) * ((float)((const uint8_t*)q.packed)[cell] * (1.0f / 255.0f));
@@ -252,6 +258,9 @@ int ssb_ply_write(const char* path, const SsbSplats* params, const SsbShQuant* s
         q = *shq;
         SSB_REQUIRE(q.bounds != nullptr, "ssb_ply_write: quantised SH needs its bounds");
         if (q.bounds_stride <= 0) q.bounds_stride = (int64_t)256 * 3 * kNumSh;
+    } else if (shq && shq->packed && shq->bits == 4) {
+        SSB_REQUIRE(((uintptr_t)shq->packed & (kShRowBytes - 1)) == 0, "ssb_ply_write: 4-bit SH rows must start on a 32-byte boundary");
+        q = *shq;
     } else {
         SSB_REQUIRE(params->features_sh != nullptr, "ssb_ply_write: features_sh is NULL and no quantised SH was given");
     }

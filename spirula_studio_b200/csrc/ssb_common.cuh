@@ -59,6 +59,10 @@ int check_loss_config(const SsbLossConfig* cfg, const char* who);
 int launch_project_bwd(const SsbSplats* splats, const SsbShQuant* shq, int64_t n, const SsbCameras* cams, const float* d_aabb,
                        SsbScreenRec* d_v_screen, const SsbSplats* grads, int accumulate, int clear_v_screen, void* stream,
                        const int32_t* d_pair_of, int64_t range_first, int64_t range_count);
+int check_shq(const SsbSplats* splats, const SsbShQuant* shq, SsbShQuant& out);
+int active_sh_count(const SsbCameras* cams);
+int launch_sh_rows_encode(const float* d_values, int64_t n, void* d_rows, cudaStream_t st);
+int launch_sh_rows_decode(const void* d_rows, int64_t n, float* d_values, cudaStream_t st);
 int launch_project_fwd_pack_pass(int pass, const SsbSplats* splats, const SsbShQuant* shq, int64_t n, const SsbCameras* cams,
                                  int32_t* d_flags, float* d_aabb, float* d_depths, float* d_radii, SsbScreenRec* d_screen,
                                  int32_t* d_camera_ids, int32_t* d_gaussian_ids, int64_t capacity, void* stream);

@@ -50,6 +50,14 @@ class SsbCameras(C.Structure):
                 ("sh_degree_plus1", C.c_int32), ("d_dist_coeffs", C.c_void_p)]
 
 
+class SsbDropout(C.Structure):
+    _fields_ = [("rate", C.c_float), ("reserved", C.c_int32), ("seed", C.c_uint64), ("offset", C.c_uint64), ("d_offset", C.c_void_p)]
+
+
+DROPPED_LOGIT = -64.0
+SH_ROW_BYTES = 32          # a splat's SH values in 4-bit codes
+
+
 class SsbLossConfig(C.Structure):
     _fields_ = [("w_l1", C.c_float), ("w_ssim", C.c_float), ("num_scales", C.c_int32), ("loss_map_mode", C.c_int32),
                 ("d_mask", C.c_void_p), ("mask_h", C.c_int32), ("mask_w", C.c_int32)]
@@ -94,6 +102,11 @@ SIGNATURES = {
     "ssb_version_string": (C.c_char_p, []),
     "ssb_project_fwd": (C.c_int, [_P, _P, _I64, _P, _P, _P, _P, _P, _P]),
     "ssb_project_bwd": (C.c_int, [_P, _P, _I64, _P, _P, _P, _P, C.c_int, _P]),
+    "ssb_sh_eval_fwd": (C.c_int, [_P, _P, _I64, _P, _P, _P]),
+    "ssb_sh_eval_bwd": (C.c_int, [_P, _P, _I64, _P, _P, _P, C.c_int, _P]),
+    "ssb_dropout": (C.c_int, [_P, _I64, _I64, _I32, _P, _P, _P]),
+    "ssb_dropout_opacities": (C.c_int, [_P, _I64, _I64, _P, _P, _P]),
+    "ssb_dropout_opacities_bwd": (C.c_int, [_P, _P, _I64, _I64, _P, _P, _P]),
     "ssb_screen_unpack": (C.c_int, [_P, _I64, _P, _P, _P, _P, _P, _P]),
     "ssb_screen_pack": (C.c_int, [_P, _P, _P, _P, _P, _I64, _P, _P]),
     "ssb_screen_unpack_add": (C.c_int, [_P, _I64, _P, _P, _P, _P, _P, _P]),
@@ -245,6 +258,14 @@ def shq_struct(packed=None, bounds=None, bits=32, bounds_stride=256):
     q.reserved = 0
     q.bounds_stride = bounds_stride
     return q
+
+
+def dropout_struct(rate, seed=0, offset=0, d_offset=None):
+    """d_offset: device int64 tensor of one word added to `offset` when a kernel runs (graph replays), or None."""
+    d = SsbDropout()
+    d.rate, d.reserved, d.seed, d.offset = rate, 0, seed, offset
+    d.d_offset = d_offset.data_ptr() if d_offset is not None else None
+    return d
 
 
 MAX_PEERS, MAX_PEER_BUFFERS, MAX_PEER_SEGMENTS, PEER_HANDLE_BYTES = 8, 4, 12, 64

@@ -73,10 +73,23 @@ class OptimOptions:
     use_per_splat_bias_correction: bool = True
 
 
+@dataclass
+class DropoutOptions:
+    """Dropout for captures with few views (ssb_dropout_opacities, ssb_dropout): every iteration each splat is left out of all
+    views with probability splat_rate, the other opacities compensated; and each group of sh_group consecutive SH values (1 a value,
+    3 a coefficient's three colours, 45 a splat's row) is left out with probability sh_rate.  The masks are functions of the seed and
+    the iteration number, the same on every rank.  Rates can change from iteration to iteration (Trainer.set_dropout).  render()
+    never drops anything."""
+    splat_rate: float = 0.0
+    sh_rate: float = 0.0
+    sh_group: int = 3
+    seed: int = 0
+
+
 class Trainer:
     def __init__(self, cfg: SceneConfig, splats: dict, device="cuda:0", isect_capacity=0, w_l1=0.8, w_ssim=0.2,
                  process_group=None, world_size=1, rank=0, grad_sync="peer", fused_backward=False, non_sh_optim_bits=32, optim=None,
-                 fused_state_layout="shared"):
+                 fused_state_layout="shared", dropout=None, view_sh_bits=32):
         self.lib = L.load()
         self.cfg = cfg
         self.device = torch.device(device)
@@ -191,6 +204,21 @@ class Trainer:
                                            optim.erank_reg, optim.erank_reg_s3, optim.quat_norm_reg, 1 if optim.use_scale_agnostic_mean else 0,
                                            self.radii.data_ptr() if self.radii is not None else None,
                                            self.steps.data_ptr() if self.steps is not None else None, n, None)
+        # What the views read in place of the stored parameters: opacities and SH values after dropout, SH values in 4-bit rows
+        # (encoded from the fp32 values before an iteration's views; the gradients are applied to the fp32 values).
+        if view_sh_bits not in (4, 32):
+            raise ValueError(f"view_sh_bits must be 32 (off) or 4; got {view_sh_bits}")
+        if view_sh_bits == 4 and self.quant:
+            raise ValueError("view_sh_bits=4 needs fp32 SH values (sh_value_bits = 32)")
+        self.view_sh_bits = view_sh_bits
+        self.dropout = None
+        self._view_opacities = self._view_sh = self._sh_rows = None
+        self._dropped = None                 # this iteration's (splat, SH) descriptions between its views and its optimiser step
+        self._v_struct, self._v_shq = self._p_struct, self.shq
+        self._views_open = False
+        if dropout is not None:
+            self.dropout = DropoutOptions(sh_group=dropout.sh_group, seed=dropout.seed)
+            self.set_dropout(dropout.splat_rate, dropout.sh_rate)
         # the range of splats whose optimiser step this rank performs
         self.first, self.count = 0, n
         if self.grad_sync in ("peer", "multimem"):
@@ -359,6 +387,7 @@ class Trainer:
         own = sum(t.numel() * t.element_size() for t in (self.params_flat, self.grads_flat, self.m1_flat, self.m2_flat))
         if self.quant:
             own += sum(t.numel() * t.element_size() for t in (self.sh_packed, self.sh_bounds, self.sh_optim_packed, self.sh_optim_bounds))
+        own += sum(t.numel() * t.element_size() for t in (self._view_opacities, self._view_sh, self._sh_rows) if t is not None)
         return own + sum(int(self.lib.ssb_step_device_bytes(h)) for h in self.handles)
 
     # -- pieces ------------------------------------------------------------
@@ -374,9 +403,79 @@ class Trainer:
             L.check(self.lib.ssb_step_set_fused_backward(self.handle, total))
             self._fused_room = total
 
-    def render(self, viewmat, intrin, kind=0, depth=False):
+    # -- what the views read -----------------------------------------------
+    def set_dropout(self, splat_rate=0.0, sh_rate=0.0):
+        """Dropout rates of the following iterations, each in [0, 1)."""
+        for rate in (splat_rate, sh_rate):
+            if not 0.0 <= rate < 1.0:
+                raise ValueError(f"dropout rates must be in [0, 1), not {rate}")
+        if (splat_rate > 0.0 or sh_rate > 0.0) and self.fused_backward:
+            raise NotImplementedError("dropout runs with the per-view backward (the fused one hands its gradients straight to the optimiser)")
+        if sh_rate > 0.0 and self.quant:
+            raise ValueError("SH dropout needs fp32 SH values (sh_value_bits = 32)")
+        if self.dropout is None:
+            self.dropout = DropoutOptions()
+        if self.dropout.sh_group < 1:
+            raise ValueError(f"sh_group must be at least 1, not {self.dropout.sh_group}")
+        self.dropout.splat_rate, self.dropout.sh_rate = float(splat_rate), float(sh_rate)
+
+    def _encode_rows(self, values, stream=None):
+        if self._sh_rows is None:
+            self._sh_rows = torch.empty(self.n * L.SH_ROW_BYTES, dtype=torch.uint8, device=self.device)
+        L.check(self.lib.ssb_quant_encode(L.ptr(values), self.n * 45, 4, L.ptr(self._sh_rows), None, stream))
+        return L.shq_struct(self._sh_rows, None, 4, 0)
+
+    def _begin_views(self, stream=None):
+        """Before an iteration's first view: makes the arrays its views read."""
+        d, i = self.dropout, self.iteration
+        self._views_open, self._dropped, self._dropped_stream = True, None, stream
+        views, shq = dict(self.params), self.shq
+        if self.quant:
+            views["features_sh"] = None
+        splat = L.dropout_struct(d.splat_rate, 2 * d.seed & 0xffffffffffffffff, i) if d is not None and d.splat_rate > 0.0 else None
+        sh = L.dropout_struct(d.sh_rate, (2 * d.seed + 1) & 0xffffffffffffffff, i) if d is not None and d.sh_rate > 0.0 else None
+        if splat is not None:
+            if self._view_opacities is None:
+                self._view_opacities = torch.empty_like(self.params["opacities"])
+            L.check(self.lib.ssb_dropout_opacities(L.ptr(self.params["opacities"]), 0, self.n, C.byref(splat), L.ptr(self._view_opacities), stream))
+            views["opacities"] = self._view_opacities
+        if sh is not None:
+            if self._view_sh is None:
+                self._view_sh = torch.empty_like(self.params["features_sh"])
+            L.check(self.lib.ssb_dropout(L.ptr(self.params["features_sh"]), 0, self.n * 45, d.sh_group, C.byref(sh), L.ptr(self._view_sh), stream))
+            views["features_sh"] = self._view_sh
+        if self.view_sh_bits == 4:
+            shq = self._encode_rows(views["features_sh"], stream)
+        if splat is not None or sh is not None:
+            self._dropped = (splat, sh, d.sh_group)
+            self._v_struct = L.splats_struct(views)
+        else:
+            self._v_struct = self._p_struct
+        self._v_shq = shq
+
+    def _end_views(self):
+        """After an iteration's last view: gradients of what the views read become gradients of the stored parameters."""
+        self._views_open = False
+        if self._dropped is None:
+            return
+        (splat, sh, group), stream = self._dropped, self._dropped_stream
+        self._dropped = None
+        if splat is not None:
+            g = self.grads["opacities"]
+            L.check(self.lib.ssb_dropout_opacities_bwd(L.ptr(self.params["opacities"]), L.ptr(g), 0, self.n, C.byref(splat), L.ptr(g), stream))
+        if sh is not None:
+            g = self.grads["features_sh"]
+            L.check(self.lib.ssb_dropout(L.ptr(g), 0, self.n * 45, group, C.byref(sh), L.ptr(g), stream))
+
+    def render(self, viewmat, intrin, kind=0, depth=False, sh_bits=None):
         """One image of the current splats, forward only (the viewer's path): viewmat [16] / intrin [4] as numpy or tensors.
-        Returns (rgb [H][W][3], transmittance [H][W]) and, with depth=True, the ray-depth image as a third tensor."""
+        Returns (rgb [H][W][3], transmittance [H][W]) and, with depth=True, the ray-depth image as a third tensor.
+        sh_bits=4 renders from the SH values in 4-bit rows (the default of a trainer whose views read them), 32 from the stored ones."""
+        sh_bits = self.view_sh_bits if sh_bits is None else sh_bits
+        if sh_bits not in (4, 32):
+            raise ValueError(f"sh_bits must be 4 or 32, not {sh_bits}")
+        if sh_bits == 4 and self.quant:
+            raise ValueError("sh_bits=4 needs fp32 SH values (sh_value_bits = 32)")
         _, _, width, height, _, _ = view_kind(self.cfg, kind)
         as_dev = lambda a, n: torch.as_tensor(np.asarray(a, np.float32) if not torch.is_tensor(a) else a, dtype=torch.float32).reshape(n).to(self.device)
         d_vm, d_K = as_dev(viewmat, 16), as_dev(intrin, 4)
@@ -384,7 +483,8 @@ class Trainer:
         T = torch.empty(height, width, device=self.device)
         dep = torch.empty(height, width, device=self.device) if depth else None
         stream = C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
-        L.check(self.lib.ssb_step_render(self.handles[kind], C.byref(self._p_struct), C.byref(self.shq) if self.shq else None, L.ptr(d_vm), L.ptr(d_K),
+        shq = self._encode_rows(self.params["features_sh"], stream) if sh_bits == 4 else self.shq
+        L.check(self.lib.ssb_step_render(self.handles[kind], C.byref(self._p_struct), C.byref(shq) if shq else None, L.ptr(d_vm), L.ptr(d_K),
                                          L.ptr(rgb), L.ptr(dep) if depth else None, L.ptr(T), stream))
         return (rgb, T, dep) if depth else (rgb, T)
 
@@ -418,13 +518,16 @@ class Trainer:
         """Forward + loss + backward of n_views views (all of camera kind `kind`) already resident on the device."""
         if self.fused_backward:
             self._keep_cams(d_viewmats, d_intrins, n_views, not accumulate)
-        L.check(self.lib.ssb_step_views(self.handles[kind], C.byref(self._p_struct), C.byref(self.shq) if self.shq else None,
+        if not accumulate or not self._views_open:
+            self._begin_views(stream)
+        L.check(self.lib.ssb_step_views(self.handles[kind], C.byref(self._v_struct), C.byref(self._v_shq) if self._v_shq else None,
                                         L.ptr(d_viewmats), L.ptr(d_intrins), L.ptr(d_gt), n_views,
                                         C.byref(self._g_struct), 1 if accumulate else 0, L.ptr(self.losses), stream))
 
     def allreduce_grads(self):
         """Makes the summed gradients available where the optimiser will read them: everywhere ("nccl"),
         or, for this rank's range of splats, in this rank's buffer ("peer")."""
+        self._end_views()
         if self.grad_sync == "nccl":
             torch.distributed.all_reduce(self.grads_flat, op=torch.distributed.ReduceOp.SUM, group=self.pg)
         elif self.grad_sync in ("peer", "multimem"):
@@ -448,6 +551,7 @@ class Trainer:
 
     def optimizer_step(self, total_views, stream=None):
         lr = self.cfg.lrs
+        self._end_views()
         self.iteration += 1
         cfg = L.SsbAdamConfig(lr["lr_means"], lr["lr_quats"], lr["lr_scales"], lr["lr_opacities"], lr["lr_features_dc"],
                               lr["lr_features_sh"], self.optim.sh_reg if self.optim is not None else 0.0, 1.0 / float(total_views), self.iteration, 0)
@@ -468,7 +572,7 @@ class Trainer:
                 layout = L.SH_LAYOUT_SPLAT_BLOCKS if self.fused_state_layout == "reference" else L.SH_LAYOUT_CELL_BLOCKS
                 sh = L.SsbShAdamState(self.sh_optim_packed.data_ptr(), self.sh_optim_bounds.data_ptr(), self.sh_packed.data_ptr(),
                                       self.sh_bounds.data_ptr(), self.cfg.sh_value_bits, 8, layout)
-            head = (self.handle, C.byref(self._p_struct), C.byref(self.shq) if self.shq else None, L.ptr(d_vm), L.ptr(d_K), int(d_vm.shape[0]))
+            head = (self.handle, C.byref(self._p_struct), C.byref(self._v_shq) if self._v_shq else None, L.ptr(d_vm), L.ptr(d_K), int(d_vm.shape[0]))
             tail = (C.byref(self._m1_struct), C.byref(self._m2_struct), C.byref(sh) if sh is not None else None, C.byref(cfg), ex, stream)
             if self._nsq is not None:
                 L.check(self.lib.ssb_step_backward_optimize_q16(*head, C.byref(self._nsq), *tail))
@@ -618,8 +722,10 @@ class Trainer:
             d_view, d_intr, d_gt = self._staging[(kind, k)]
             if self.fused_backward:
                 self._keep_cams(d_view, d_intr, nv, first)
+            if first:
+                self._begin_views()
             # one call per camera kind: each view's loss stage waits on the device for its own target
-            L.check(self.lib.ssb_step_views_gated(self.handles[kind], C.byref(self._p_struct), C.byref(self.shq) if self.shq else None,
+            L.check(self.lib.ssb_step_views_gated(self.handles[kind], C.byref(self._v_struct), C.byref(self._v_shq) if self._v_shq else None,
                                                   L.ptr(d_view), L.ptr(d_intr), L.ptr(d_gt), nv, handles,
                                                   C.byref(self._g_struct), 0 if first else 1, L.ptr(self.losses), None))
             first = False

@@ -1,0 +1,457 @@
+"""Dropout, 4-bit SH rows and the SH product on the device against their 64-bit statements, through the C ABI."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import view_ops_oracle as O  # noqa: E402
+from spirula_studio_b200 import lib as L  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+SEED, OFFSET = 0x9182736455463728, (7 << 32) + 12345
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    return L.load()
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).to(DEV)
+
+
+def shifted(n, shift, fill=7.0):
+    """A view of n floats that starts `shift` floats behind a 256-byte boundary, in a buffer of a known value."""
+    buf = torch.full((n + shift + 64,), fill, device=DEV)
+    return buf, buf[shift:shift + n]
+
+
+def untouched(buf, view, fill=7.0):
+    mask = torch.ones_like(buf, dtype=torch.bool)
+    off = (view.data_ptr() - buf.data_ptr()) // 4
+    mask[off:off + view.numel()] = False
+    return bool((buf[mask] == fill).all())
+
+
+def within(got, want, tol):
+    got = got.detach().cpu().numpy().astype(np.float64).reshape(np.shape(want))
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:3].tolist(), got[bad][:3], np.asarray(want)[bad][:3], np.broadcast_to(tol, got.shape)[bad][:3])
+
+
+# ---- dropout ----------------------------------------------------------------------------------------------------------
+
+# y = x * fl(1 / (1 - r)): two roundings
+DROPOUT_RTOL = 2 * O.U * (1 + 2.0 ** -20)
+
+
+@pytest.mark.parametrize("count", [1, 2, 3, 4, 5, 17, 255, 1000, 4099, 70001])
+@pytest.mark.parametrize("group,first", [(1, 0), (1, 3), (2, 5), (3, 0), (3, 7), (4, 1), (5, 2), (9, 100), (45, 0), (45, 46), (1000, 999)])
+def test_dropout_matches_the_oracle(lib, count, group, first):
+    rng = np.random.default_rng(count * 131 + group)
+    x = rng.normal(size=count).astype(np.float32)
+    for rate, sx, sy in ((0.1, 0, 0), (0.5, 1, 2), (0.999, 3, 3)):
+        d = L.dropout_struct(rate, SEED, OFFSET)
+        bx, vx = shifted(count, sx)
+        by, vy = shifted(count, sy)
+        vx.copy_(torch.from_numpy(x))
+        L.check(lib.ssb_dropout(L.ptr(vx), first, count, group, C.byref(d), L.ptr(vy), None))
+        torch.cuda.synchronize()
+        want = O.dropout(x, first, group, rate, SEED, OFFSET)
+        got = vy.cpu().numpy()
+        assert np.array_equal(got == 0, want == 0)
+        within(vy, want, DROPOUT_RTOL * np.abs(want))
+        assert untouched(by, vy) and untouched(bx, vx)
+
+
+def test_dropout_in_place_and_as_its_own_backward(lib):
+    x = np.random.default_rng(3).normal(size=45 * 301).astype(np.float32)
+    d = L.dropout_struct(0.3, 5, 9)
+    t = dev(x)
+    L.check(lib.ssb_dropout(L.ptr(t), 0, t.numel(), 3, C.byref(d), L.ptr(t), None))
+    want = O.dropout(x, 0, 3, 0.3, 5, 9)
+    within(t, want, DROPOUT_RTOL * np.abs(want))
+    # <dropout(x), v> = <x, dropout(v)>
+    v = dev(np.random.default_rng(4).normal(size=x.size).astype(np.float32))
+    gv = torch.empty_like(v)
+    L.check(lib.ssb_dropout(L.ptr(v), 0, v.numel(), 3, C.byref(d), L.ptr(gv), None))
+    a, b = (t.double() * v.double()).sum().item(), (dev(x).double() * gv.double()).sum().item()
+    assert abs(a - b) <= 2 * DROPOUT_RTOL * (t.double() * v.double()).abs().sum().item()
+
+
+def test_dropout_does_not_look_at_dropped_values(lib):
+    n = 4096
+    dropped = O.dropped(0, n, 1, 0.4, SEED, OFFSET)
+    x = np.ones(n, np.float32)
+    x[dropped] = np.tile(np.array([np.nan, np.inf, -np.inf, np.finfo(np.float32).min], np.float32), n)[:dropped.sum()]
+    t = dev(x)
+    d = L.dropout_struct(0.4, SEED, OFFSET)
+    y = torch.empty_like(t)
+    L.check(lib.ssb_dropout(L.ptr(t), 0, n, 1, C.byref(d), L.ptr(y), None))
+    y = y.cpu().numpy()
+    assert np.all(y[dropped] == 0) and np.all(y[~dropped] == np.float32(1 / (1 - float(np.float32(0.4)))))
+    kept = np.where(dropped, np.float32(1), np.float32(np.nan))
+    L.check(lib.ssb_dropout(L.ptr(dev(kept)), 0, n, 1, C.byref(d), L.ptr(t), None))
+    assert np.array_equal(np.isnan(t.cpu().numpy()), ~dropped)
+
+
+def test_dropout_rate_zero_keeps_every_bit_and_shards_agree(lib):
+    x = np.random.default_rng(8).normal(size=10007).astype(np.float32)
+    x[:3] = np.nan, np.inf, -0.0
+    t, y = dev(x), torch.empty(10007, device=DEV)
+    d = L.dropout_struct(0.0, SEED, OFFSET)
+    L.check(lib.ssb_dropout(L.ptr(t), 0, x.size, 1, C.byref(d), L.ptr(y), None))
+    assert np.array_equal(y.cpu().numpy().view(np.uint32)[1:], x.view(np.uint32)[1:]) and np.isnan(y[0].item())
+    d = L.dropout_struct(0.25, SEED, OFFSET)
+    whole, parts = torch.empty_like(t), torch.empty_like(t)
+    L.check(lib.ssb_dropout(L.ptr(t), 0, x.size, 3, C.byref(d), L.ptr(whole), None))
+    for a, b in ((0, 1), (1, 4000), (4000, 4001), (4001, 10007)):
+        L.check(lib.ssb_dropout(C.c_void_p(t.data_ptr() + 4 * a), a, b - a, 3, C.byref(d), C.c_void_p(parts.data_ptr() + 4 * a), None))
+    assert torch.equal(whole.view(torch.int32), parts.view(torch.int32))
+
+
+def test_dropout_group_numbers_beyond_32_bits(lib):
+    x = np.random.default_rng(8).normal(size=5000).astype(np.float32)
+    t, y = dev(x), torch.empty(5000, device=DEV)
+    d = L.dropout_struct(0.5, SEED, OFFSET)
+    for first in (2 ** 32 - 6, 2 ** 34 - 2501, 2 ** 40 + 1, 2 ** 62 - 5000):
+        for group in (1, 3, 45):
+            L.check(lib.ssb_dropout(L.ptr(t), first, x.size, group, C.byref(d), L.ptr(y), None))
+            want = O.dropout(x, first, group, 0.5, SEED, OFFSET)
+            assert np.array_equal(y.cpu().numpy() == 0, want == 0), (first, group)
+    L.check(lib.ssb_dropout_opacities(L.ptr(t), 2 ** 34 - 2501, x.size, C.byref(d), L.ptr(y), None))
+    assert np.array_equal(y.cpu().numpy() == O.DROPPED, O.dropped(2 ** 34 - 2501, 5000, 1, 0.5, SEED, OFFSET))
+
+
+def test_dropout_rate_is_the_rate(lib):
+    n = 1 << 22
+    x = torch.ones(n, device=DEV)
+    for rate in (0.01, 0.37, 0.9):
+        d = L.dropout_struct(rate, 1, 2)
+        L.check(lib.ssb_dropout(L.ptr(x), 0, n, 1, C.byref(d), L.ptr(y := torch.empty_like(x)), None))
+        # the masks are fixed by (seed, offset): a six sigma band of the binomial count
+        assert abs((y == 0).sum().item() - rate * n) <= 6 * (n * rate * (1 - rate)) ** 0.5
+
+
+# ---- opacities --------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rate", [0.0, 1e-30, 1e-6, 0.01, 0.1, 0.5, 0.9, 0.9999])
+@pytest.mark.parametrize("count,first,shift", [(1, 0, 0), (3, 5, 1), (1000, 0, 3), (40001, 12345, 2)])
+def test_opacities_forward_and_backward(lib, rate, count, first, shift):
+    rng = np.random.default_rng(count)
+    x = rng.normal(size=count).astype(np.float32) * np.where(rng.random(count) < 0.3, 6.0, 1.0).astype(np.float32)
+    r = float(np.float32(rate))
+    if count > 100 and r > 0:
+        # next to the limit, where 1 - z cancels, and at both ends
+        edge = np.log(O.CAP * (1 - r) / (1 - O.CAP * (1 - r)))
+        x[10:60] = (edge + np.linspace(-1e-3, 1e-3, 50)).astype(np.float32)
+        x[60:68] = [80, -80, 1e30, -1e30, np.inf, -np.inf, 0.0, -88.0]
+    v = rng.normal(size=count).astype(np.float32)
+    d = L.dropout_struct(rate, SEED, OFFSET)
+    bx, vx = shifted(count, shift)
+    by, vy = shifted(count, shift)
+    bg, vg = shifted(count, shift)
+    vx.copy_(torch.from_numpy(x))
+    L.check(lib.ssb_dropout_opacities(L.ptr(vx), first, count, C.byref(d), L.ptr(vy), None))
+    L.check(lib.ssb_dropout_opacities_bwd(L.ptr(vx), L.ptr(dev(v)), first, count, C.byref(d), L.ptr(vg), None))
+    torch.cuda.synchronize()
+    y, slope, bound = O.dropout_opacities(x, first, rate, SEED, OFFSET)
+    if r == 0.0:
+        assert torch.equal(vy, vx) and torch.equal(vg, dev(v))
+        return
+    got = vy.cpu().numpy().astype(np.float64)
+    inf = ~np.isfinite(y)
+    assert np.array_equal(got[inf], y[inf])
+    within(torch.from_numpy(got[~inf]), y[~inf], bound[~inf])
+    # w off by 4 U, a quotient of two ulps (4 U)
+    within(vg, slope * v, 8 * O.U * np.abs(slope * v))
+    assert np.array_equal(vg.cpu().numpy()[slope == 0], np.zeros(int((slope == 0).sum()), np.float32))
+    for b, t in ((bx, vx), (by, vy), (bg, vg)):
+        assert untouched(b, t)
+
+
+def test_opacities_nan_stays_nan_unless_dropped_and_in_place(lib):
+    n = 2000
+    d = L.dropout_struct(0.5, 1, 1)
+    t = torch.full((n,), float("nan"), device=DEV)
+    y = torch.empty_like(t)
+    L.check(lib.ssb_dropout_opacities(L.ptr(t), 0, n, C.byref(d), L.ptr(y), None))
+    drop = O.dropped(0, n, 1, 0.5, 1, 1)
+    y = y.cpu().numpy()
+    assert np.all(y[drop] == O.DROPPED) and np.all(np.isnan(y[~drop]))
+    x = np.random.default_rng(0).normal(size=n).astype(np.float32)
+    a, b = dev(x), torch.empty(n, device=DEV)
+    L.check(lib.ssb_dropout_opacities(L.ptr(a), 0, n, C.byref(d), L.ptr(b), None))
+    c = a.clone()
+    L.check(lib.ssb_dropout_opacities(L.ptr(c), 0, n, C.byref(d), L.ptr(c), None))
+    assert torch.equal(b, c)
+    v = dev(np.random.default_rng(1).normal(size=n).astype(np.float32))
+    g = torch.empty_like(v)
+    L.check(lib.ssb_dropout_opacities_bwd(L.ptr(a), L.ptr(v), 0, n, C.byref(d), L.ptr(g), None))
+    L.check(lib.ssb_dropout_opacities_bwd(L.ptr(a), L.ptr(v), 0, n, C.byref(d), L.ptr(v), None))
+    assert torch.equal(g, v)
+
+
+def test_dropout_graph_replays_draw_new_masks(lib):
+    n = 45 * 1000
+    x = dev(np.random.default_rng(0).normal(size=n).astype(np.float32))
+    y, o = torch.empty_like(x), torch.empty(1000, device=DEV)
+    word = torch.zeros(1, dtype=torch.int64, device=DEV)
+    d = L.dropout_struct(0.3, 11, 100, word)
+    s = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        st = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+        L.check(lib.ssb_dropout(L.ptr(x), 0, n, 3, C.byref(d), L.ptr(y), st))
+        L.check(lib.ssb_dropout_opacities(L.ptr(x), 0, 1000, C.byref(d), L.ptr(o), st))
+        word.add_(1)
+    for k in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(y.cpu().numpy() == 0, O.dropped(0, n, 3, 0.3, 11, 100 + k))
+        assert np.array_equal(o.cpu().numpy() == O.DROPPED, O.dropped(0, 1000, 1, 0.3, 11, 100 + k))
+
+
+# ---- 4-bit rows -------------------------------------------------------------------------------------------------------
+
+def row_inputs(n, seed=0):
+    rng = np.random.default_rng(seed)
+    sh = (0.05 * rng.normal(size=(n, 15, 3))).astype(np.float32)
+    sh[rng.random(n) < 0.1] = 0.0
+    sh[rng.random(n) < 0.1, 8:] = 0.0                     # bands not trained yet
+    sh *= np.exp2(rng.integers(-8, 6, size=(n, 1, 1))).astype(np.float32)
+    return sh
+
+
+def encode(lib, sh):
+    n = sh.shape[0]
+    rows = torch.full((n, 32), 0xa5, dtype=torch.uint8, device=DEV)
+    L.check(lib.ssb_quant_encode(L.ptr(sh), n * 45, 4, L.ptr(rows), None, None))
+    return rows
+
+
+def decode(lib, rows):
+    n = rows.shape[0]
+    out = torch.full((n, 15, 3), 9.0, device=DEV)
+    L.check(lib.ssb_quant_decode(L.ptr(rows), None, n * 45, 4, L.ptr(out), None))
+    torch.cuda.synchronize()
+    return out
+
+
+@pytest.mark.parametrize("n", [1, 2, 31, 32, 127, 128, 129, 1000, 20011])
+@pytest.mark.parametrize("shift", [0, 1, 2])
+def test_rows_equal_the_oracle_bit_for_bit(lib, n, shift):
+    sh = row_inputs(n, n)
+    buf, v = shifted(n * 45, shift)
+    v.copy_(torch.from_numpy(sh.reshape(-1)))
+    rows = encode(lib, v.view(n, 15, 3))
+    q, s = O.encode_rows(sh)
+    assert np.array_equal(rows.cpu().numpy(), O.pack_rows(q, s))
+    ob, ov = shifted(n * 45, shift)
+    L.check(lib.ssb_quant_decode(L.ptr(rows), None, n * 45, 4, L.ptr(ov), None))
+    torch.cuda.synchronize()
+    assert np.array_equal(ov.cpu().numpy(), O.row_values(q, s).astype(np.float32).reshape(-1))
+    assert untouched(ob, ov) and untouched(buf, v)
+
+
+def test_rows_of_awkward_values(lib):
+    f = np.float32
+    sh = np.zeros((16, 15, 3), f)
+    sh[0, 0, 0] = np.nan
+    sh[1, 0] = (np.inf, -np.inf, 1.0)
+    sh[2, 3:8] = np.inf                                   # nothing finite in the band
+    sh[3] = f(1e-45)                                      # denormals: no scale
+    sh[4] = f(2.0 ** -100); sh[5] = np.nextafter(f(2.0 ** -100), f(0))
+    sh[6] = np.finfo(f).max; sh[7] = -np.finfo(f).max
+    # midpoints: ties to even, and one step to either side of each
+    for k in range(15):
+        sh[8, k, 0] = (k - 7) * 0.5; sh[8, k, 1] = np.nextafter(f((k - 7) * 0.5), f(9)); sh[8, k, 2] = np.nextafter(f((k - 7) * 0.5), f(-9))
+    sh[8, (0, 3, 8), 0] = 7.0
+    sh[9] = 7.0 * 1.0078125                               # exactly seven bf16 steps
+    sh[10] = np.nextafter(f(7.0 * 1.0078125), f(8))       # just above: the next bf16
+    sh[11] = -0.0
+    rng = np.random.default_rng(2)
+    sh[12:] = (rng.integers(-15, 16, size=(4, 15, 3)) * 0.5).astype(f)
+    rows = encode(lib, dev(sh))
+    q, s = O.encode_rows(sh)
+    assert np.array_equal(rows.cpu().numpy(), O.pack_rows(q, s))
+    assert np.array_equal(decode(lib, rows).cpu().numpy(), O.row_values(q, s).astype(f))
+    zero = torch.zeros(5, 32, dtype=torch.uint8, device=DEV)
+    assert not decode(lib, zero).any()
+
+
+# ---- the product ------------------------------------------------------------------------------------------------------
+
+def cameras(views, seed=0, far=0.0):
+    rng = np.random.default_rng(seed)
+    vm = np.zeros((views, 4, 4))
+    for v in range(views):
+        R, _ = np.linalg.qr(rng.normal(size=(3, 3)))
+        c = 6.0 * rng.normal(size=3) + far
+        vm[v, :3, :3], vm[v, :3, 3], vm[v, 3, 3] = R, -R @ c, 1
+    return vm.reshape(views, 16).astype(np.float32)
+
+
+def sources(lib, sh, fmt):
+    """(SsbShQuant or None, fp32 features or None, the values they stand for, tensors to keep alive)."""
+    n = sh.shape[0]
+    if fmt == 32:
+        t = dev(sh)
+        return None, t, sh.astype(np.float64), [t]
+    if fmt == 4:
+        rows = encode(lib, dev(sh))
+        return L.shq_struct(rows, None, 4, 0), None, O.row_values(*O.encode_rows(sh)), [rows]
+    t = dev(sh.reshape(-1))
+    packed = torch.zeros(n * 45 * fmt // 8, dtype=torch.uint8, device=DEV)
+    bounds = torch.zeros((n * 45 + 255) // 256 * 2, device=DEV)
+    L.check(lib.ssb_quant_encode(L.ptr(t), n * 45, fmt, L.ptr(packed), L.ptr(bounds), None))
+    vals = torch.empty(n * 45, device=DEV)
+    L.check(lib.ssb_quant_decode(L.ptr(packed), L.ptr(bounds), n * 45, fmt, L.ptr(vals), None))
+    return L.shq_struct(packed, bounds, fmt, 256), None, vals.cpu().numpy().astype(np.float64).reshape(n, 15, 3), [packed, bounds]
+
+
+def eval_case(n, views, seed=0, far=0.0):
+    rng = np.random.default_rng(seed + n)
+    return dict(means=(4 * rng.normal(size=(n, 3)) + far).astype(np.float32), dc=(0.3 * rng.normal(size=(n, 3))).astype(np.float32),
+                sh=(0.05 * rng.normal(size=(n, 15, 3))).astype(np.float32), vm=cameras(views, seed, far),
+                v=rng.normal(size=(views, n, 3)).astype(np.float32))
+
+
+def run_fwd(lib, c, src, degree=3, with_dc=True, shift=0, stream=None):
+    shq, feat = src[0], src[1]
+    n, views = len(c["means"]), len(c["vm"])
+    m, dc, vm = dev(c["means"]), dev(c["dc"]), dev(c["vm"])
+    s = L.splats_struct(dict(means=m, features_dc=dc if with_dc else None, features_sh=feat))
+    cams = L.cameras_struct(vm, vm, 1, 1, sh_degree=degree)
+    buf, out = shifted(views * n * 3, shift)
+    L.check(lib.ssb_sh_eval_fwd(C.byref(s), C.byref(shq) if shq else None, n, C.byref(cams), L.ptr(out), stream))
+    torch.cuda.synchronize()
+    assert untouched(buf, out)
+    return out.view(views, n, 3)
+
+
+def run_bwd(lib, c, src, degree=3, accumulate=0, base=None, want=("means", "features_dc", "features_sh"), shift=0):
+    shq, feat = src[0], src[1]
+    n = len(c["means"])
+    m, dc, vm, v = dev(c["means"]), dev(c["dc"]), dev(c["vm"]), dev(c["v"])
+    s = L.splats_struct(dict(means=m, features_dc=dc, features_sh=feat))
+    cams = L.cameras_struct(vm, vm, 1, 1, sh_degree=degree)
+    bufs = {k: shifted(n * w, shift) for k, w in (("means", 3), ("features_dc", 3), ("features_sh", 45))}
+    if base is not None:
+        for k, t in base.items():
+            bufs[k][1].copy_(t.reshape(-1))
+    g = L.splats_struct({k: bufs[k][1] for k in want})
+    L.check(lib.ssb_sh_eval_bwd(C.byref(s), C.byref(shq) if shq else None, n, C.byref(cams), L.ptr(v), C.byref(g), accumulate, None))
+    torch.cuda.synchronize()
+    assert all(untouched(*b) for b in bufs.values())
+    return {k: bufs[k][1] for k in bufs}
+
+
+@pytest.mark.parametrize("fmt", [4, 8, 16, 32])
+@pytest.mark.parametrize("n,views,degree,shift", [(1, 1, 3, 0), (5, 2, 2, 1), (127, 1, 3, 2), (128, 3, 3, 0), (129, 1, 1, 3), (1000, 16, 3, 1),
+                                                  (1000, 1, 0, 0), (4001, 33, 3, 0), (300, 70, 2, 0), (20003, 1, 3, 1), (20004, 1, 3, 0)])
+def test_eval_forward_and_backward(lib, fmt, n, views, degree, shift):
+    c = eval_case(n, views)
+    src = sources(lib, c["sh"], fmt)
+    want, tol = O.sh_eval(c["means"], c["dc"], src[2], c["vm"], degree)
+    within(run_fwd(lib, c, src, degree, shift=shift), want, tol)
+    (gm, gd, gs), (tm, td, ts) = O.sh_eval_bwd(c["means"], src[2], c["vm"], c["v"], degree)
+    g = run_bwd(lib, c, src, degree, shift=shift)
+    within(g["means"], gm, tm); within(g["features_dc"], gd, td); within(g["features_sh"], gs, ts)
+    # added to what is there: one more rounding
+    base = {k: torch.randn(t.numel(), device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)) for k, t in g.items()}
+    a = run_bwd(lib, c, src, degree, accumulate=1, base=base, shift=shift)
+    for k, w, t in (("means", gm, tm), ("features_dc", gd, td), ("features_sh", gs, ts)):
+        b = base[k].cpu().numpy().astype(np.float64).reshape(w.shape)
+        within(a[k], w + b, t + O.U * (np.abs(w + b) + t))
+
+
+def test_eval_without_dc_and_with_unwanted_gradients(lib):
+    c = eval_case(500, 3)
+    src = sources(lib, c["sh"], 4)
+    want, tol = O.sh_eval(c["means"], None, src[2], c["vm"])
+    within(run_fwd(lib, c, src, with_dc=False), want, tol)
+    whole = run_bwd(lib, c, src)
+    for keep in (("means",), ("features_dc",), ("features_sh",), ("means", "features_sh"), ()):
+        g = run_bwd(lib, c, src, want=keep)
+        for k in g:
+            assert torch.equal(g[k], whole[k]) if k in keep else bool((g[k] == 7.0).all())
+
+
+def test_eval_degree_zero_needs_no_sh_values(lib):
+    c = eval_case(300, 2)
+    out = run_fwd(lib, c, (None, None), degree=0)
+    want = np.broadcast_to(O.C0 * c["dc"].astype(np.float64), (2, 300, 3))
+    within(out, want, 2 * O.U * np.abs(want))
+    g = run_bwd(lib, c, (None, None), degree=0)
+    assert not g["means"].any() and not g["features_sh"].any()
+
+
+def test_eval_no_views_gives_zero_gradients(lib):
+    c = eval_case(200, 1)
+    c["vm"], c["v"] = np.zeros((0, 16), np.float32), np.zeros((0, 200, 3), np.float32)
+    src = sources(lib, c["sh"], 4)
+    g = run_bwd(lib, c, src)
+    assert not any(t.any() for t in g.values())
+
+
+def test_eval_far_from_the_origin_and_at_the_camera(lib):
+    """Positions of thousands with cameras a few units away; then splats at the camera's centre, extremely near and far ones."""
+    c = eval_case(400, 2, seed=3, far=4000.0)
+    src = sources(lib, c["sh"], 4)
+    want, tol = O.sh_eval(c["means"], c["dc"], src[2], c["vm"])
+    within(run_fwd(lib, c, src), want, tol)
+    (gm, gd, gs), (tm, td, ts) = O.sh_eval_bwd(c["means"], src[2], c["vm"], c["v"])
+    g = run_bwd(lib, c, src)
+    within(g["means"], gm, tm); within(g["features_sh"], gs, ts)
+    c = eval_case(8, 1)
+    c["vm"] = np.eye(4, dtype=np.float32).reshape(1, 16)
+    c["means"][:] = [[0, 0, 0], [1e-30, 0, 2e-30], [3e25, -4e25, 0], [0, 0, 1e-20], [0, -1e18, 1], [1e-10, 2e-10, -1e-10], [0, 0, -5], [1, 2, 3]]
+    src = sources(lib, c["sh"], 4)
+    want, tol = O.sh_eval(c["means"], c["dc"], src[2], c["vm"])
+    within(run_fwd(lib, c, src), want, tol)
+    within(run_fwd(lib, c, src)[0, :1], O.C0 * c["dc"][:1].astype(np.float64), 2 * O.U * np.abs(c["dc"][:1]))
+    (gm, gd, gs), (tm, td, ts) = O.sh_eval_bwd(c["means"], src[2], c["vm"], c["v"])
+    g = run_bwd(lib, c, src)
+    assert not g["means"].view(8, 3)[0].any() and not g["features_sh"].view(8, 45)[0].any()
+    within(g["means"], gm, tm); within(g["features_sh"], gs, ts)
+
+
+def test_eval_on_another_stream_and_in_a_graph(lib):
+    c = eval_case(1000, 4)
+    src = sources(lib, c["sh"], 4)
+    ref = run_fwd(lib, c, src)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    assert torch.equal(run_fwd(lib, c, src, stream=C.c_void_p(s.cuda_stream)), ref)
+    m, dc, vm, v = dev(c["means"]), dev(c["dc"]), dev(c["vm"]), dev(c["v"])
+    sp = L.splats_struct(dict(means=m, features_dc=dc))
+    cams = L.cameras_struct(vm, vm, 1, 1)
+    sh = dev(c["sh"])
+    rows = torch.zeros(1000, 32, dtype=torch.uint8, device=DEV)
+    shq = L.shq_struct(rows, None, 4, 0)
+    out = torch.zeros(4, 1000, 3, device=DEV)
+    gm, gs = torch.zeros(1000, 3, device=DEV), torch.zeros(1000, 45, device=DEV)
+    gr = L.splats_struct(dict(means=gm, features_sh=gs))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        st = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+        L.check(lib.ssb_quant_encode(L.ptr(sh), 45000, 4, L.ptr(rows), None, st))
+        L.check(lib.ssb_sh_eval_fwd(C.byref(sp), C.byref(shq), 1000, C.byref(cams), L.ptr(out), st))
+        L.check(lib.ssb_sh_eval_bwd(C.byref(sp), C.byref(shq), 1000, C.byref(cams), L.ptr(v), C.byref(gr), 0, st))
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, ref)
+    whole = run_bwd(lib, c, src)
+    assert torch.equal(gm.view(-1), whole["means"]) and torch.equal(gs.view(-1), whole["features_sh"])
+    sh.mul_(-1)                                            # new values, same graph
+    g.replay()
+    torch.cuda.synchronize()
+    c2 = dict(c, sh=-c["sh"])
+    assert torch.equal(out, run_fwd(lib, c2, sources(lib, c2["sh"], 4)))
