@@ -31,15 +31,89 @@ __device__ __forceinline__ uint64_t drop_offset(const DropArgs& a) { return a.of
 __device__ __forceinline__ uint4 drop_words(const DropArgs& a, uint64_t offset, uint64_t block) {
     return philox4x32_10(make_uint4((uint32_t)block, (uint32_t)(block >> 32), (uint32_t)offset, (uint32_t)(offset >> 32)), a.key0, a.key1);
 }
-__device__ __forceinline__ uint32_t word_of(const uint4& w, int k) { return k == 0 ? w.x : (k == 1 ? w.y : (k == 2 ? w.z : w.w)); }
+// Four consecutive values at p[i], of which only those with 0 <= i + k < count exist.  VEC: p + i is 16-byte aligned.
+template <bool VEC>
+__device__ __forceinline__ float4 load4(const float* p, int64_t i, int64_t count) {
+    if (VEC && i >= 0 && i + 3 < count) return *(const float4*)(p + i);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (i >= 0 && i < count) v.x = p[i];
+    if (i + 1 >= 0 && i + 1 < count) v.y = p[i + 1];
+    if (i + 2 >= 0 && i + 2 < count) v.z = p[i + 2];
+    if (i + 3 >= 0 && i + 3 < count) v.w = p[i + 3];
+    return v;
+}
+template <bool VEC>
+__device__ __forceinline__ void store4(float* p, int64_t i, int64_t count, float4 v) {
+    if (VEC && i >= 0 && i + 3 < count) { *(float4*)(p + i) = v; return; }
+    if (i >= 0 && i < count) p[i] = v.x;
+    if (i + 1 >= 0 && i + 1 < count) p[i + 1] = v.y;
+    if (i + 2 >= 0 && i + 2 < count) p[i + 2] = v.z;
+    if (i + 3 >= 0 && i + 3 < count) p[i + 3] = v.w;
+}
 
-__global__ void __launch_bounds__(256) dropout_kernel(const float* x, float* y, int64_t first, int64_t count, int32_t group,
-                                                      DropArgs a) {
+constexpr int kDropThreads = 256;
+constexpr int kDropChunks = 4;                                     // chunks of four values per thread, all loads in flight
+constexpr int kDropTile = kDropThreads * kDropChunks * 4;          // values per block
+
+// Every value decides for itself: a thread's four values are the four words of one generator block, so the decisions never
+// leave registers.  Chunks start on multiples of four of the whole array's numbering.
+template <bool VEC>
+__global__ void __launch_bounds__(kDropThreads) dropout_values_kernel(const float* x, float* y, int64_t first, int64_t count, DropArgs a) {
     const uint64_t offset = drop_offset(a);
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
-        const uint64_t g = (uint64_t)(first + i) / (uint32_t)group;
-        const uint32_t w = word_of(drop_words(a, offset, g >> 2), (int)(g & 3));
-        y[i] = w < a.threshold ? 0.0f : x[i] * a.scale;
+    const int64_t chunk0 = (int64_t)blockIdx.x * (kDropThreads * kDropChunks) + threadIdx.x;
+    const int64_t i0 = 4 * chunk0 - (first & 3);
+    float4 v[kDropChunks];
+#pragma unroll
+    for (int c = 0; c < kDropChunks; ++c) v[c] = load4<VEC>(x, i0 + 4 * kDropThreads * c, count);
+#pragma unroll
+    for (int c = 0; c < kDropChunks; ++c) {
+        const uint4 w = drop_words(a, offset, (uint64_t)(first >> 2) + (uint64_t)(chunk0 + kDropThreads * c));
+        v[c].x = w.x < a.threshold ? 0.0f : v[c].x * a.scale;
+        v[c].y = w.y < a.threshold ? 0.0f : v[c].y * a.scale;
+        v[c].z = w.z < a.threshold ? 0.0f : v[c].z * a.scale;
+        v[c].w = w.w < a.threshold ? 0.0f : v[c].w * a.scale;
+        store4<VEC>(y, i0 + 4 * kDropThreads * c, count, v[c]);
+    }
+}
+
+// Groups of several values: the decisions of the groups that a block's tile touches are made once, one generator block per
+// four groups, and kept as one byte each in shared memory while the tile's values are on their way.
+struct GroupArgs { uint32_t group, magic; int32_t shift; };        // shift: values before the first 16-byte boundary of x, negated start of tile 0
+
+template <bool VEC>
+__global__ void __launch_bounds__(kDropThreads) dropout_groups_kernel(const float* x, float* y, int64_t first, int64_t count, GroupArgs ga, DropArgs a) {
+    __shared__ uint32_t keep_s[(kDropTile / 2 + 8) / 4 + 2];
+    const uint64_t offset = drop_offset(a);
+    const int64_t tile = (int64_t)blockIdx.x * kDropTile - ga.shift;            // the tile's first value; may lie before the array
+    const int64_t i0 = tile + 4 * threadIdx.x;
+    float4 v[kDropChunks];
+#pragma unroll
+    for (int c = 0; c < kDropChunks; ++c) v[c] = load4<VEC>(x, i0 + 4 * kDropThreads * c, count);
+    const int64_t lo = max(tile, (int64_t)0), hi = min(tile + kDropTile, count) - 1;
+    const uint64_t g0 = (uint64_t)(first + lo) / ga.group;
+    const uint32_t r0 = (uint32_t)((uint64_t)(first + lo) - g0 * ga.group);     // place of value lo in its group
+    const uint32_t span = (uint32_t)(hi - lo) + r0;                             // place of value hi, counted from the start of group g0
+    const uint32_t n_groups = (span < ga.group ? 0 : (ga.magic ? __umulhi(span, ga.magic) : 1)) + 1;
+    const uint32_t lead = (uint32_t)(g0 & 3);
+    for (uint32_t b = threadIdx.x; 4 * b < lead + n_groups; b += kDropThreads) {
+        const uint4 w = drop_words(a, offset, (g0 >> 2) + b);
+        keep_s[b] = (w.x < a.threshold ? 0u : 1u) | (w.y < a.threshold ? 0u : 1u << 8) | (w.z < a.threshold ? 0u : 1u << 16) |
+                    (w.w < a.threshold ? 0u : 1u << 24);
+    }
+    __syncthreads();
+    const uint8_t* keep = (const uint8_t*)keep_s + lead;
+#pragma unroll
+    for (int c = 0; c < kDropChunks; ++c) {
+        const int64_t i = i0 + 4 * kDropThreads * c;
+        float* e = &v[c].x;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            // values outside the array take some decision of the tile: they are not stored
+            const uint32_t p = i + k < lo || i + k > hi ? 0u : (uint32_t)(i + k - lo) + r0;
+            const uint32_t q = ga.magic ? __umulhi(p, ga.magic) : (p >= ga.group ? 1u : 0u);
+            e[k] = keep[q] ? e[k] * a.scale : 0.0f;
+        }
+        store4<VEC>(y, i, count, v[c]);
     }
 }
 
@@ -54,17 +128,28 @@ struct OpacityArgs {
 };
 
 template <bool BWD>
-__global__ void __launch_bounds__(256) dropout_opacity_kernel(const float* x, const float* v, float* out,
-                                                              int64_t first, int64_t count, DropArgs a, OpacityArgs o) {
-    const uint64_t offset = drop_offset(a);
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
-        const uint64_t g = (uint64_t)(first + i);
-        const bool dropped = word_of(drop_words(a, offset, g >> 2), (int)(g & 3)) < a.threshold;
-        const float xi = x[i];
-        const float w = -expm1f(-((o.x0_hi - xi) + o.x0_lo));
-        if (BWD) out[i] = (dropped || xi > o.x_cap) ? 0.0f : v[i] / w;
-        else out[i] = dropped ? kDroppedLogit : (xi > o.x_cap ? o.capped : (xi + o.a) - logf(w));
-    }
+__device__ __forceinline__ float drop_opacity(float x, float v, bool dropped, const OpacityArgs& o) {
+    const float w = -expm1f(-((o.x0_hi - x) + o.x0_lo));
+    if (BWD) return (dropped || x > o.x_cap) ? 0.0f : v / w;
+    return dropped ? kDroppedLogit : (x > o.x_cap ? o.capped : (x + o.a) - logf(w));
+}
+
+template <bool BWD, bool VEC>
+__global__ void __launch_bounds__(kDropThreads) dropout_opacity_kernel(const float* x, const float* v, float* out, int64_t first, int64_t count,
+                                                                       DropArgs a, OpacityArgs o) {
+    const int64_t chunk = (int64_t)blockIdx.x * kDropThreads + threadIdx.x;
+    const int64_t i = 4 * chunk - (first & 3);
+    if (i >= count) return;
+    const float4 xv = load4<VEC>(x, i, count);
+    float4 vv = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (BWD) vv = load4<VEC>(v, i, count);
+    const uint4 w = drop_words(a, drop_offset(a), (uint64_t)(first >> 2) + (uint64_t)chunk);
+    float4 r;
+    r.x = drop_opacity<BWD>(xv.x, vv.x, w.x < a.threshold, o);
+    r.y = drop_opacity<BWD>(xv.y, vv.y, w.y < a.threshold, o);
+    r.z = drop_opacity<BWD>(xv.z, vv.z, w.z < a.threshold, o);
+    r.w = drop_opacity<BWD>(xv.w, vv.w, w.w < a.threshold, o);
+    store4<VEC>(out, i, count, r);
 }
 
 static int drop_args(const SsbDropout* d, const char* who, DropArgs* a) {
@@ -81,7 +166,7 @@ static int drop_args(const SsbDropout* d, const char* who, DropArgs* a) {
 }
 
 static int check_range(int64_t first, int64_t count, const char* who) {
-    SSB_REQUIRE(first >= 0 && count >= 0 && first <= ((int64_t)1 << 62) && count <= ((int64_t)1 << 62) - first, "%s: bad range", who);
+    SSB_REQUIRE(first >= 0 && count >= 0 && first <= ((int64_t)1 << 62) && count <= ((int64_t)1 << 40), "%s: bad range", who);
     return SSB_OK;
 }
 
@@ -90,8 +175,6 @@ static int check_floats(const char* who, const void* a, const void* b, const voi
     SSB_REQUIRE((((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & 3) == 0, "%s: arrays must lie on 4-byte boundaries", who);
     return SSB_OK;
 }
-
-static unsigned drop_blocks(int64_t count) { return (unsigned)(count > 148 * 8 * 256 ? 148 * 8 : ceil_div(count, 256)); }
 
 static OpacityArgs opacity_args(float rate) {
     const double r = rate, cap = 0.999;
@@ -108,6 +191,22 @@ static OpacityArgs opacity_args(float rate) {
     return o;
 }
 
+// Whether value `first` being at p leaves the multiples of four of the numbering on 16-byte boundaries.
+static bool chunk_aligned(const void* p, int64_t first) { return (((uintptr_t)p >> 2) & 3) == (uintptr_t)(first & 3); }
+
+static int launch_opacity(bool bwd, const float* x, const float* v, float* out, int64_t first, int64_t count, const SsbDropout* d, const DropArgs& a,
+                          cudaStream_t st) {
+    const unsigned blocks = (unsigned)ceil_div(count + (first & 3), 4 * kDropThreads);
+    const OpacityArgs o = opacity_args(d->rate);
+    const bool vec = chunk_aligned(x, first) && chunk_aligned(out, first) && (!bwd || chunk_aligned(v, first));
+    if (bwd && vec) dropout_opacity_kernel<true, true><<<blocks, kDropThreads, 0, st>>>(x, v, out, first, count, a, o);
+    else if (bwd) dropout_opacity_kernel<true, false><<<blocks, kDropThreads, 0, st>>>(x, v, out, first, count, a, o);
+    else if (vec) dropout_opacity_kernel<false, true><<<blocks, kDropThreads, 0, st>>>(x, v, out, first, count, a, o);
+    else dropout_opacity_kernel<false, false><<<blocks, kDropThreads, 0, st>>>(x, v, out, first, count, a, o);
+    SSB_LAUNCHED("dropout_opacity_kernel");
+    return SSB_OK;
+}
+
 }  // namespace ssb
 
 extern "C" {
@@ -120,8 +219,25 @@ int ssb_dropout(const float* d_x, int64_t first, int64_t count, int32_t group, c
     SSB_REQUIRE(group >= 1, "ssb_dropout: group must be at least 1 (got %d)", group);
     if (count == 0) return SSB_OK;
     if (int e = check_floats("ssb_dropout", d_x, d_x, d_y)) return e;
-    dropout_kernel<<<drop_blocks(count), 256, 0, (cudaStream_t)stream>>>(d_x, d_y, first, count, group, a);
-    SSB_LAUNCHED("dropout_kernel");
+    cudaStream_t st = (cudaStream_t)stream;
+    if (group == 1) {
+        const unsigned blocks = (unsigned)ceil_div(count + (first & 3), kDropTile);
+        if (chunk_aligned(d_x, first) && chunk_aligned(d_y, first)) dropout_values_kernel<true><<<blocks, kDropThreads, 0, st>>>(d_x, d_y, first, count, a);
+        else dropout_values_kernel<false><<<blocks, kDropThreads, 0, st>>>(d_x, d_y, first, count, a);
+        SSB_LAUNCHED("dropout_values_kernel");
+        return SSB_OK;
+    }
+    // p / group = umulhi(p, ceil(2^32 / group)) for p < group + kDropTile as long as group (group + kDropTile) < 2^32; a tile
+    // touches at most two larger groups
+    const bool vec = (((uintptr_t)d_x ^ (uintptr_t)d_y) & 15) == 0;
+    GroupArgs ga;
+    ga.group = (uint32_t)group;
+    ga.magic = group <= 32768 ? (uint32_t)(((uint64_t)1 << 32) / (uint32_t)group + 1) : 0;
+    ga.shift = vec ? (int32_t)(((uintptr_t)d_x >> 2) & 3) : 0;
+    const unsigned blocks = (unsigned)ceil_div(count + ga.shift, kDropTile);
+    if (vec) dropout_groups_kernel<true><<<blocks, kDropThreads, 0, st>>>(d_x, d_y, first, count, ga, a);
+    else dropout_groups_kernel<false><<<blocks, kDropThreads, 0, st>>>(d_x, d_y, first, count, ga, a);
+    SSB_LAUNCHED("dropout_groups_kernel");
     return SSB_OK;
 }
 
@@ -136,9 +252,7 @@ int ssb_dropout_opacities(const float* d_opacities, int64_t first, int64_t count
         if (d_out != d_opacities) SSB_CUDA(cudaMemcpyAsync(d_out, d_opacities, (size_t)count * sizeof(float), cudaMemcpyDeviceToDevice, (cudaStream_t)stream));
         return SSB_OK;
     }
-    dropout_opacity_kernel<false><<<drop_blocks(count), 256, 0, (cudaStream_t)stream>>>(d_opacities, nullptr, d_out, first, count, a, opacity_args(dropout->rate));
-    SSB_LAUNCHED("dropout_opacity_kernel");
-    return SSB_OK;
+    return launch_opacity(false, d_opacities, nullptr, d_out, first, count, dropout, a, (cudaStream_t)stream);
 }
 
 int ssb_dropout_opacities_bwd(const float* d_opacities, const float* d_v_out, int64_t first, int64_t count, const SsbDropout* dropout,
@@ -153,9 +267,7 @@ int ssb_dropout_opacities_bwd(const float* d_opacities, const float* d_v_out, in
         if (d_v_out != d_v_opacities) SSB_CUDA(cudaMemcpyAsync(d_v_opacities, d_v_out, (size_t)count * sizeof(float), cudaMemcpyDeviceToDevice, (cudaStream_t)stream));
         return SSB_OK;
     }
-    dropout_opacity_kernel<true><<<drop_blocks(count), 256, 0, (cudaStream_t)stream>>>(d_opacities, d_v_out, d_v_opacities, first, count, a, opacity_args(dropout->rate));
-    SSB_LAUNCHED("dropout_opacity_kernel");
-    return SSB_OK;
+    return launch_opacity(true, d_opacities, d_v_out, d_v_opacities, first, count, dropout, a, (cudaStream_t)stream);
 }
 
 }  // extern "C"
