@@ -2,6 +2,8 @@
 // coefficient matrix with the basis of its viewing directions, forward and backward.
 #include "sh_device.cuh"
 
+#include <algorithm>
+
 namespace ssb {
 
 // ---- 4-bit rows -------------------------------------------------------------
@@ -28,37 +30,65 @@ __device__ __forceinline__ int row_code(float v, float s, float inv) {
 }
 
 __global__ void __launch_bounds__(kProjBlock) sh_rows_encode_kernel(const float* __restrict__ sh, int64_t n, uint4* __restrict__ rows) {
-    const int64_t i = (int64_t)blockIdx.x * kProjBlock + threadIdx.x;
+    __shared__ __align__(16) float sh_s[kProjBlock * kShPerSplat];
+    const int64_t first = (int64_t)blockIdx.x * kProjBlock;
+    const int64_t i = first + threadIdx.x;
+    stage_sh(sh_s, nullptr, sh, nullptr, nullptr, 32, 256, first, n);
+    __syncthreads();
     if (i >= n) return;
-    const float* v = sh + kShPerSplat * i;
-    float s[3], inv[3];
+    float v[kShPerSplat];
 #pragma unroll
-    for (int b = 0; b < 3; ++b) {
-        float m = 0.0f;
-        for (int j = 0; j < kNumSh; ++j)
-            if (sh_band(j) == b)
-                for (int ch = 0; ch < 3; ++ch) {
-                    const float a = fabsf(v[3 * j + ch]);
-                    m = fmaxf(m, a <= 3.402823466e38f ? a : 0.0f);
-                }
-        s[b] = row_scale(m);
-        inv[b] = s[b] > 0.0f ? 1.0f / s[b] : 0.0f;
+    for (int k = 0; k < kShPerSplat; ++k) v[k] = sh_s[threadIdx.x * kShPerSplat + k];
+    float m[3] = {0.0f, 0.0f, 0.0f}, s[3], inv[3];
+#pragma unroll
+    for (int k = 0; k < kShPerSplat; ++k) {
+        const float a = fabsf(v[k]);
+        m[sh_band(k / 3)] = fmaxf(m[sh_band(k / 3)], a <= 3.402823466e38f ? a : 0.0f);
     }
+#pragma unroll
+    for (int b = 0; b < 3; ++b) { s[b] = row_scale(m[b]); inv[b] = s[b] > 0.0f ? 1.0f / s[b] : 0.0f; }
     uint32_t w[8] = {};
+#pragma unroll
     for (int j = 0; j < kNumSh; ++j)
-        for (int ch = 0; ch < 3; ++ch) {
-            const int b = sh_band(j);
-            w[2 * ch + (j >> 3)] |= (uint32_t)(row_code(v[3 * j + ch], s[b], inv[b]) + 8) << (4 * (j & 7));
-        }
+#pragma unroll
+        for (int ch = 0; ch < 3; ++ch)
+            w[2 * ch + (j >> 3)] |= (uint32_t)(row_code(v[3 * j + ch], s[sh_band(j)], inv[sh_band(j)]) + 8) << (4 * (j & 7));
     w[6] = (__float_as_uint(s[0]) >> 16) | (__float_as_uint(s[1]) & 0xffff0000u);
     w[7] = __float_as_uint(s[2]) >> 16;
     rows[2 * i] = make_uint4(w[0], w[1], w[2], w[3]);
     rows[2 * i + 1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
+// Writes a block's contiguous span of `count` floats from shared memory (16-byte aligned there) to global memory.  A full span
+// on a 16-byte boundary leaves as one bulk copy (or, when added to what is there, one bulk reduction: every address belongs to one
+// thread block, so the sum has one order); anything else takes coalesced 4-byte stores.  All threads call it between the barrier
+// after the span was written and bulk_done().
+__device__ __forceinline__ void store_span(float* dst, const float* span_s, int count, int full, bool add) {
+    if (count == full && ((uintptr_t)dst & 15) == 0) {
+        if (threadIdx.x == 0) {
+            const uint32_t src = (uint32_t)__cvta_generic_to_shared(span_s);
+            if (add) asm volatile("cp.reduce.async.bulk.global.shared::cta.bulk_group.add.f32 [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(4 * full) : "memory");
+            else asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(4 * full) : "memory");
+        }
+    } else if (add) for (int k = threadIdx.x; k < count; k += kProjBlock) dst[k] += span_s[k];
+    else for (int k = threadIdx.x; k < count; k += kProjBlock) dst[k] = span_s[k];
+}
+// The thread's writes to shared memory become visible to bulk copies issued after the next barrier.
+__device__ __forceinline__ void span_written() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// Waits until the block's bulk copies have read their spans (the spans may then be written again, or the block may end).
+__device__ __forceinline__ void bulk_done() {
+    if (threadIdx.x == 0) asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+
 __global__ void __launch_bounds__(kProjBlock) sh_rows_decode_kernel(const void* __restrict__ rows, int64_t n, float* __restrict__ sh) {
-    const int64_t i = (int64_t)blockIdx.x * kProjBlock + threadIdx.x;
-    if (i < n) decode_sh_row(load_sh_row(rows, i), sh + kShPerSplat * i);
+    __shared__ __align__(16) float sh_s[kProjBlock * kShPerSplat];
+    const int64_t first = (int64_t)blockIdx.x * kProjBlock;
+    const int64_t i = first + threadIdx.x;
+    if (i < n) decode_sh_row(load_sh_row(rows, i), sh_s + threadIdx.x * kShPerSplat);
+    span_written();
+    __syncthreads();
+    store_span(sh + first * kShPerSplat, sh_s, (int)min((int64_t)kProjBlock, n - first) * kShPerSplat, kProjBlock * kShPerSplat, false);
+    bulk_done();
 }
 
 int launch_sh_rows_encode(const float* d_values, int64_t n, void* d_rows, cudaStream_t st) {
@@ -113,89 +143,145 @@ __device__ __forceinline__ Direction view_direction(const ViewCentre& c, const f
     return {dx * inv, dy * inv, dz * inv, inv};
 }
 
+constexpr int kCentreChunk = 32;      // views whose centres a block keeps at a time
+
+__device__ __forceinline__ void stage_centres(ViewCentre* centres_s, const float* __restrict__ viewmats, int v0, int views) {
+    const int v = v0 + threadIdx.x;
+    if (threadIdx.x < kCentreChunk && v < views) centres_s[threadIdx.x] = view_centre(viewmats, v);
+}
+
+// The SH values of the thread's splat: in registers from its 4-bit row, or from the block's staged span.
+template <bool ROWS>
+__device__ __forceinline__ void read_sh(float sh[kShPerSplat], const float* sh_s, const SsbShQuant& shq, int64_t i, int n_sh) {
+    if (n_sh == 0) {
+#pragma unroll
+        for (int k = 0; k < kShPerSplat; ++k) sh[k] = 0.0f;
+    } else if (ROWS) {
+        decode_sh_row(load_sh_row(shq.packed, i), sh);
+    } else {
+#pragma unroll
+        for (int k = 0; k < kShPerSplat; ++k) sh[k] = sh_s[threadIdx.x * kShPerSplat + k];
+    }
+}
+
 template <bool ROWS>
 __global__ void __launch_bounds__(kProjBlock) sh_eval_fwd_kernel(SsbSplats sp, SsbShQuant shq, int64_t n, int views, const float* __restrict__ viewmats,
                                                                  int n_sh, float* __restrict__ out) {
-    __shared__ __align__(16) float sh_s[kProjBlock * kShPerSplat];
+    __shared__ __align__(16) float sh_s[ROWS ? 4 : kProjBlock * kShPerSplat];
     __shared__ __align__(16) unsigned char raw_s[ROWS ? 16 : kShRawBytes];
-    const int64_t first = (int64_t)blockIdx.x * kProjBlock;
-    const int64_t i = first + threadIdx.x;
-    if (n_sh > 0) {
-        stage_sh(sh_s, raw_s, sp.features_sh, shq.packed, shq.bounds, ROWS ? 4 : shq.bits, shq.bounds_stride, first, n);
-        __syncthreads();
-    }
-    if (i >= n) return;
-    const float mean[3] = {sp.means[3 * i], sp.means[3 * i + 1], sp.means[3 * i + 2]};
-    float dc[3] = {0.f, 0.f, 0.f};
-    if (sp.features_dc) for (int ch = 0; ch < 3; ++ch) dc[ch] = kShC0 * sp.features_dc[3 * i + ch];
-    const float* sh = sh_s + threadIdx.x * kShPerSplat;
-    for (int v = 0; v < views; ++v) {
-        const Direction d = view_direction(view_centre(viewmats, v), mean);
-        float b[kNumSh];
-        sh_basis(d.x, d.y, d.z, b);
-        if (d.inv == 0.0f) b[5] = 0.0f;            // no direction: the one basis function that does not vanish by itself
-        float c[3] = {dc[0], dc[1], dc[2]};
+    __shared__ ViewCentre centres_s[kCentreChunk];
+    stage_centres(centres_s, viewmats, 0, views);
+    __syncthreads();
+    for (int64_t first = (int64_t)blockIdx.x * kProjBlock; first < n; first += (int64_t)gridDim.x * kProjBlock) {
+        const int64_t i = first + threadIdx.x;
+        if (!ROWS && n_sh > 0) {
+            __syncthreads();
+            stage_sh(sh_s, raw_s, sp.features_sh, shq.packed, shq.bounds, shq.bits, shq.bounds_stride, first, n);
+            __syncthreads();
+        }
+        const int64_t il = min(i, n - 1);
+        const float mean[3] = {sp.means[3 * il], sp.means[3 * il + 1], sp.means[3 * il + 2]};
+        float dc[3] = {0.f, 0.f, 0.f};
+        if (sp.features_dc)
 #pragma unroll
-        for (int j = 0; j < kNumSh; ++j)
-            if (j < n_sh)
+            for (int ch = 0; ch < 3; ++ch) dc[ch] = kShC0 * sp.features_dc[3 * il + ch];
+        float sh[kShPerSplat];
+        read_sh<ROWS>(sh, sh_s, shq, il, n_sh);
+        for (int v0 = 0; v0 < views; v0 += kCentreChunk) {
+            if (views > kCentreChunk) {
+                __syncthreads();
+                stage_centres(centres_s, viewmats, v0, views);
+                __syncthreads();
+            }
+            const int v1 = min(views - v0, kCentreChunk);
+            for (int v = 0; v < v1; ++v) {
+                const Direction d = view_direction(centres_s[v], mean);
+                float b[kNumSh];
+                sh_basis(d.x, d.y, d.z, b);
+                if (d.inv == 0.0f) b[5] = 0.0f;            // no direction: the one basis function that does not vanish by itself
+                float c[3] = {dc[0], dc[1], dc[2]};
 #pragma unroll
-                for (int ch = 0; ch < 3; ++ch) c[ch] += b[j] * sh[3 * j + ch];
-        float* o = out + 3 * ((int64_t)v * n + i);
-        o[0] = c[0]; o[1] = c[1]; o[2] = c[2];
+                for (int j = 0; j < kNumSh; ++j)
+                    if (j < n_sh)
+#pragma unroll
+                        for (int ch = 0; ch < 3; ++ch) c[ch] += b[j] * sh[3 * j + ch];
+                if (i < n) {
+                    float* o = out + 3 * ((int64_t)(v0 + v) * n + i);
+                    o[0] = c[0]; o[1] = c[1]; o[2] = c[2];
+                }
+            }
+        }
     }
 }
 
 template <bool ROWS>
 __global__ void __launch_bounds__(kProjBlock) sh_eval_bwd_kernel(SsbSplats sp, SsbShQuant shq, int64_t n, int views, const float* __restrict__ viewmats,
                                                                  int n_sh, const float* __restrict__ v_out, SsbSplats gr, int accumulate) {
-    __shared__ __align__(16) float sh_s[kProjBlock * kShPerSplat];
+    __shared__ __align__(16) float sh_s[kProjBlock * kShPerSplat];       // values on the way in, their gradients on the way out
+    __shared__ __align__(16) float mean_s[kProjBlock * 3];
+    __shared__ __align__(16) float dc_s[kProjBlock * 3];
     __shared__ __align__(16) unsigned char raw_s[ROWS ? 16 : kShRawBytes];
-    const int64_t first = (int64_t)blockIdx.x * kProjBlock;
-    const int64_t i = first + threadIdx.x;
-    if (n_sh > 0) {
-        stage_sh(sh_s, raw_s, sp.features_sh, shq.packed, shq.bounds, ROWS ? 4 : shq.bits, shq.bounds_stride, first, n);
+    __shared__ ViewCentre centres_s[kCentreChunk];
+    stage_centres(centres_s, viewmats, 0, views);
+    for (int64_t first = (int64_t)blockIdx.x * kProjBlock; first < n; first += (int64_t)gridDim.x * kProjBlock) {
+        const int64_t i = first + threadIdx.x, il = min(i, n - 1);
         __syncthreads();
-    }
-    if (i >= n) return;
-    const float mean[3] = {sp.means[3 * i], sp.means[3 * i + 1], sp.means[3 * i + 2]};
-    const float* sh = sh_s + threadIdx.x * kShPerSplat;
-    float g_mean[3] = {0.f, 0.f, 0.f}, g_dc[3] = {0.f, 0.f, 0.f}, g_sh[kShPerSplat];
+        if (!ROWS && n_sh > 0) {
+            stage_sh(sh_s, raw_s, sp.features_sh, shq.packed, shq.bounds, shq.bits, shq.bounds_stride, first, n);
+            __syncthreads();
+        }
+        const float mean[3] = {sp.means[3 * il], sp.means[3 * il + 1], sp.means[3 * il + 2]};
+        float sh[kShPerSplat], g_mean[3] = {0.f, 0.f, 0.f}, g_dc[3] = {0.f, 0.f, 0.f}, g_sh[kShPerSplat];
+        read_sh<ROWS>(sh, sh_s, shq, il, n_sh);
 #pragma unroll
-    for (int k = 0; k < kShPerSplat; ++k) g_sh[k] = 0.f;
-    for (int v = 0; v < views; ++v) {
-        const float* gp = v_out + 3 * ((int64_t)v * n + i);
-        const float g[3] = {gp[0], gp[1], gp[2]};
-        const Direction d = view_direction(view_centre(viewmats, v), mean);
-        float b[kNumSh], w[kNumSh];
-        sh_basis(d.x, d.y, d.z, b);
-        if (d.inv == 0.0f) b[5] = 0.0f;            // no direction: the one basis function that does not vanish by itself
+        for (int k = 0; k < kShPerSplat; ++k) g_sh[k] = 0.f;
+        for (int v0 = 0; v0 < views; v0 += kCentreChunk) {
+            if (views > kCentreChunk) {
+                __syncthreads();
+                stage_centres(centres_s, viewmats, v0, views);
+                __syncthreads();
+            }
+            const int v1 = min(views - v0, kCentreChunk);
+            for (int v = 0; v < v1; ++v) {
+                const float* gp = v_out + 3 * ((int64_t)(v0 + v) * n + il);
+                const float g[3] = {gp[0], gp[1], gp[2]};
+                const Direction d = view_direction(centres_s[v], mean);
+                float b[kNumSh], w[kNumSh];
+                sh_basis(d.x, d.y, d.z, b);
+                if (d.inv == 0.0f) b[5] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < kNumSh; ++j) {
-            w[j] = 0.0f;
-            if (j < n_sh) {
+                for (int j = 0; j < kNumSh; ++j) {
+                    w[j] = 0.0f;
+                    if (j < n_sh) {
 #pragma unroll
-                for (int ch = 0; ch < 3; ++ch) { w[j] += sh[3 * j + ch] * g[ch]; g_sh[3 * j + ch] += b[j] * g[ch]; }
+                        for (int ch = 0; ch < 3; ++ch) { w[j] += sh[3 * j + ch] * g[ch]; g_sh[3 * j + ch] += b[j] * g[ch]; }
+                    }
+                }
+#pragma unroll
+                for (int ch = 0; ch < 3; ++ch) g_dc[ch] += kShC0 * g[ch];
+                float vn[3];
+                sh_basis_vjp(d.x, d.y, d.z, w, vn);
+                const float dn = d.x * vn[0] + d.y * vn[1] + d.z * vn[2];
+                g_mean[0] += (vn[0] - d.x * dn) * d.inv;
+                g_mean[1] += (vn[1] - d.y * dn) * d.inv;
+                g_mean[2] += (vn[2] - d.z * dn) * d.inv;
             }
         }
+        bulk_done();
+        __syncthreads();          // the previous tile's copies have left, and every thread has read its values
 #pragma unroll
-        for (int ch = 0; ch < 3; ++ch) g_dc[ch] += kShC0 * g[ch];
-        float vn[3];
-        sh_basis_vjp(d.x, d.y, d.z, w, vn);
-        const float dn = d.x * vn[0] + d.y * vn[1] + d.z * vn[2];
-        g_mean[0] += (vn[0] - d.x * dn) * d.inv;
-        g_mean[1] += (vn[1] - d.y * dn) * d.inv;
-        g_mean[2] += (vn[2] - d.z * dn) * d.inv;
-    }
+        for (int k = 0; k < 3; ++k) { mean_s[3 * threadIdx.x + k] = g_mean[k]; dc_s[3 * threadIdx.x + k] = g_dc[k]; }
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-        if (gr.means) gr.means[3 * i + k] = accumulate ? gr.means[3 * i + k] + g_mean[k] : g_mean[k];
-        if (gr.features_dc) gr.features_dc[3 * i + k] = accumulate ? gr.features_dc[3 * i + k] + g_dc[k] : g_dc[k];
+        for (int k = 0; k < kShPerSplat; ++k) sh_s[kShPerSplat * threadIdx.x + k] = g_sh[k];
+        span_written();
+        __syncthreads();
+        const int count = (int)min((int64_t)kProjBlock, n - first);
+        if (gr.means) store_span(gr.means + 3 * first, mean_s, 3 * count, 3 * kProjBlock, accumulate != 0);
+        if (gr.features_dc) store_span(gr.features_dc + 3 * first, dc_s, 3 * count, 3 * kProjBlock, accumulate != 0);
+        if (gr.features_sh) store_span(gr.features_sh + kShPerSplat * first, sh_s, kShPerSplat * count, kProjBlock * kShPerSplat, accumulate != 0);
+        if (!ROWS) bulk_done();   // the next tile is staged into the same span
     }
-    if (gr.features_sh) {
-        float* o = gr.features_sh + kShPerSplat * i;
-#pragma unroll
-        for (int k = 0; k < kShPerSplat; ++k) o[k] = accumulate ? o[k] + g_sh[k] : g_sh[k];
-    }
+    bulk_done();
 }
 
 // Checks shared by the two directions; on success q is the SH source and *n_sh the coefficients past DC in use.
@@ -225,7 +311,7 @@ int ssb_sh_eval_fwd(const SsbSplats* splats, const SsbShQuant* shq, int64_t n, c
     if (int e = check_eval(splats, shq, n, cams, "ssb_sh_eval_fwd", &q, &n_sh)) return e;
     if (n == 0 || cams->count == 0) return SSB_OK;
     SSB_REQUIRE(d_values && ((uintptr_t)d_values & 3) == 0, "ssb_sh_eval_fwd: d_values is NULL or not on a 4-byte boundary");
-    const unsigned blocks = (unsigned)ceil_div(n, kProjBlock);
+    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(n, kProjBlock), 148 * 8);
     if (q.bits == 4) sh_eval_fwd_kernel<true><<<blocks, kProjBlock, 0, (cudaStream_t)stream>>>(*splats, q, n, cams->count, cams->d_viewmats, n_sh, d_values);
     else sh_eval_fwd_kernel<false><<<blocks, kProjBlock, 0, (cudaStream_t)stream>>>(*splats, q, n, cams->count, cams->d_viewmats, n_sh, d_values);
     SSB_LAUNCHED("sh_eval_fwd_kernel");
@@ -243,7 +329,7 @@ int ssb_sh_eval_bwd(const SsbSplats* splats, const SsbShQuant* shq, int64_t n, c
     SSB_REQUIRE(d_v_values || cams->count == 0, "ssb_sh_eval_bwd: NULL argument");
     SSB_REQUIRE((((uintptr_t)d_v_values | (uintptr_t)grads->means | (uintptr_t)grads->features_dc | (uintptr_t)grads->features_sh) & 3) == 0,
                 "ssb_sh_eval_bwd: arrays must lie on 4-byte boundaries");
-    const unsigned blocks = (unsigned)ceil_div(n, kProjBlock);
+    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(n, kProjBlock), 148 * 8);
     if (q.bits == 4) sh_eval_bwd_kernel<true><<<blocks, kProjBlock, 0, (cudaStream_t)stream>>>(*splats, q, n, cams->count, cams->d_viewmats, n_sh, d_v_values, *grads, accumulate);
     else sh_eval_bwd_kernel<false><<<blocks, kProjBlock, 0, (cudaStream_t)stream>>>(*splats, q, n, cams->count, cams->d_viewmats, n_sh, d_v_values, *grads, accumulate);
     SSB_LAUNCHED("sh_eval_bwd_kernel");
