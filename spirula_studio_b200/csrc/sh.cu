@@ -29,6 +29,18 @@ __device__ __forceinline__ int row_code(float v, float s, float inv) {
     return (int)q;
 }
 
+// The row's six words of codes, value by value as row_code defines them; `sh` holds the splat's 45 values.
+__device__ __noinline__ void encode_row_checked(const float* sh, uint32_t w[6], const float s[3], const float inv[3]) {
+    for (int j = 0; j < kNumSh; ++j)
+        for (int ch = 0; ch < 3; ++ch) {
+            const int k = 2 * ch + (j >> 3);
+            w[k] = ((j & 7) ? w[k] : 0u) | (uint32_t)(row_code(sh[3 * j + ch], s[sh_band(j)], inv[sh_band(j)]) + 8) << (4 * (j & 7));
+        }
+}
+
+// Per value: t = v / s + 8 + 1.5 2^23 rounds to the code and leaves it in the low bits of t, so a word is a sum of shifted t's less
+// a constant.  The remainder decides whether the rounding was the right one (see row_code); rows with a value next to a midpoint,
+// an infinity or a NaN -- one splat in a hundred thousand of ordinary ones -- take the checked way.
 __global__ void __launch_bounds__(kProjBlock) sh_rows_encode_kernel(const float* __restrict__ sh, int64_t n, uint4* __restrict__ rows) {
     __shared__ __align__(16) float sh_s[kProjBlock * kShPerSplat];
     const int64_t first = (int64_t)blockIdx.x * kProjBlock;
@@ -39,20 +51,44 @@ __global__ void __launch_bounds__(kProjBlock) sh_rows_encode_kernel(const float*
     float v[kShPerSplat];
 #pragma unroll
     for (int k = 0; k < kShPerSplat; ++k) v[k] = sh_s[threadIdx.x * kShPerSplat + k];
-    float m[3] = {0.0f, 0.0f, 0.0f}, s[3], inv[3];
+    float m[3] = {0.0f, 0.0f, 0.0f}, s[3], inv[3], half[3], odd = 0.0f;
 #pragma unroll
     for (int k = 0; k < kShPerSplat; ++k) {
-        const float a = fabsf(v[k]);
-        m[sh_band(k / 3)] = fmaxf(m[sh_band(k / 3)], a <= 3.402823466e38f ? a : 0.0f);
+        m[sh_band(k / 3)] = fmaxf(m[sh_band(k / 3)], fabsf(v[k]));
+        odd = fmaf(v[k], 0.0f, odd);                     // NaN as soon as one value is not finite
+    }
+    bool checked = odd != 0.0f;
+    if (checked) {
+        m[0] = m[1] = m[2] = 0.0f;
+        for (int k = 0; k < kShPerSplat; ++k) {
+            const float a = fabsf(sh_s[threadIdx.x * kShPerSplat + k]), f = a <= 3.402823466e38f ? a : 0.0f;
+            if (k < 9) m[0] = fmaxf(m[0], f); else if (k < 24) m[1] = fmaxf(m[1], f); else m[2] = fmaxf(m[2], f);
+        }
     }
 #pragma unroll
-    for (int b = 0; b < 3; ++b) { s[b] = row_scale(m[b]); inv[b] = s[b] > 0.0f ? 1.0f / s[b] : 0.0f; }
+    for (int b = 0; b < 3; ++b) {
+        s[b] = row_scale(m[b]);
+        inv[b] = s[b] > 0.0f ? 1.0f / s[b] : 0.0f;
+        half[b] = s[b] > 0.0f ? 0.5f * s[b] : INFINITY;
+    }
+    constexpr float kMagic = 12582912.0f + 8.0f;
     uint32_t w[8] = {};
 #pragma unroll
     for (int j = 0; j < kNumSh; ++j)
 #pragma unroll
-        for (int ch = 0; ch < 3; ++ch)
-            w[2 * ch + (j >> 3)] |= (uint32_t)(row_code(v[3 * j + ch], s[sh_band(j)], inv[sh_band(j)]) + 8) << (4 * (j & 7));
+        for (int ch = 0; ch < 3; ++ch) {
+            const float x = v[3 * j + ch], t = fmaf(x, inv[sh_band(j)], kMagic);
+            checked |= fabsf(fmaf(kMagic - t, s[sh_band(j)], x)) >= half[sh_band(j)];
+            w[2 * ch + (j >> 3)] += __float_as_uint(t) << (4 * (j & 7));
+        }
+#pragma unroll
+    for (int ch = 0; ch < 3; ++ch) { w[2 * ch] -= 0x4b400000u * 0x11111111u; w[2 * ch + 1] -= 0x4b400000u * 0x01111111u; }
+    if (checked) {
+        uint32_t c[6];
+        encode_row_checked(sh_s + threadIdx.x * kShPerSplat, c, s, inv);
+#pragma unroll
+        for (int k = 0; k < 6; ++k) w[k] = c[k];
+    }
     w[6] = (__float_as_uint(s[0]) >> 16) | (__float_as_uint(s[1]) & 0xffff0000u);
     w[7] = __float_as_uint(s[2]) >> 16;
     rows[2 * i] = make_uint4(w[0], w[1], w[2], w[3]);
