@@ -160,22 +160,30 @@ __device__ __forceinline__ float drop_opacity(float x, float v, bool dropped, co
     return dropped ? kDroppedLogit : (x > o.x_cap ? o.capped : (x + o.a) - logf(w));
 }
 
+constexpr int kOpacityChunks = 2;
+
 template <bool BWD, bool VEC>
 __global__ void __launch_bounds__(kDropThreads) dropout_opacity_kernel(const float* x, const float* v, float* out, int64_t first, int64_t count,
                                                                        DropArgs a, OpacityArgs o) {
-    const int64_t chunk = (int64_t)blockIdx.x * kDropThreads + threadIdx.x;
-    const int64_t i = 4 * chunk - (first & 3);
-    if (i >= count) return;
-    const float4 xv = load4<VEC>(x, i, count);
-    float4 vv = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (BWD) vv = load4<VEC>(v, i, count);
-    const uint4 w = drop_words(a, drop_offset(a), (uint64_t)(first >> 2) + (uint64_t)chunk);
-    float4 r;
-    r.x = drop_opacity<BWD>(xv.x, vv.x, w.x < a.threshold, o);
-    r.y = drop_opacity<BWD>(xv.y, vv.y, w.y < a.threshold, o);
-    r.z = drop_opacity<BWD>(xv.z, vv.z, w.z < a.threshold, o);
-    r.w = drop_opacity<BWD>(xv.w, vv.w, w.w < a.threshold, o);
-    store4<VEC>(out, i, count, r);
+    const uint64_t offset = drop_offset(a);
+    const int64_t chunk0 = (int64_t)blockIdx.x * (kDropThreads * kOpacityChunks) + threadIdx.x;
+    const int64_t i0 = 4 * chunk0 - (first & 3);
+    float4 xv[kOpacityChunks], vv[kOpacityChunks];
+#pragma unroll
+    for (int c = 0; c < kOpacityChunks; ++c) {
+        xv[c] = load4<VEC>(x, i0 + 4 * kDropThreads * c, count);
+        if (BWD) vv[c] = load4<VEC>(v, i0 + 4 * kDropThreads * c, count);
+    }
+#pragma unroll
+    for (int c = 0; c < kOpacityChunks; ++c) {
+        const uint4 w = drop_words(a, offset, (uint64_t)(first >> 2) + (uint64_t)(chunk0 + kDropThreads * c));
+        float4 r;
+        r.x = drop_opacity<BWD>(xv[c].x, BWD ? vv[c].x : 0.f, w.x < a.threshold, o);
+        r.y = drop_opacity<BWD>(xv[c].y, BWD ? vv[c].y : 0.f, w.y < a.threshold, o);
+        r.z = drop_opacity<BWD>(xv[c].z, BWD ? vv[c].z : 0.f, w.z < a.threshold, o);
+        r.w = drop_opacity<BWD>(xv[c].w, BWD ? vv[c].w : 0.f, w.w < a.threshold, o);
+        store4<VEC>(out, i0 + 4 * kDropThreads * c, count, r);
+    }
 }
 
 static int drop_args(const SsbDropout* d, const char* who, DropArgs* a) {
@@ -222,7 +230,7 @@ static bool chunk_aligned(const void* p, int64_t first) { return (((uintptr_t)p 
 
 static int launch_opacity(bool bwd, const float* x, const float* v, float* out, int64_t first, int64_t count, const SsbDropout* d, const DropArgs& a,
                           cudaStream_t st) {
-    const unsigned blocks = (unsigned)ceil_div(count + (first & 3), 4 * kDropThreads);
+    const unsigned blocks = (unsigned)ceil_div(count + (first & 3), 4 * kDropThreads * kOpacityChunks);
     const OpacityArgs o = opacity_args(d->rate);
     const bool vec = chunk_aligned(x, first) && chunk_aligned(out, first) && (!bwd || chunk_aligned(v, first));
     if (bwd && vec) dropout_opacity_kernel<true, true><<<blocks, kDropThreads, 0, st>>>(x, v, out, first, count, a, o);

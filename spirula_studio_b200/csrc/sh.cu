@@ -142,87 +142,313 @@ int launch_sh_rows_decode(const void* d_rows, int64_t n, float* d_values, cudaSt
 }
 
 // ---- the product ------------------------------------------------------------
-// value[v][i] = C0 dc_i + sum_j b_j(dir) W_i[j], dir = (mean_i - centre_v) / |mean_i - centre_v|.  The difference is what
-// loses bits when a camera is close to a splat far from the origin, so the centre is kept as a sum of two floats.
-struct ViewCentre { float hi[3], lo[3]; };     // -centre = R^T t
+// value[v][i] = C0 dc_i + sum_j b_j(dir) W_i[j], dir = (mean_i - centre_v) / |mean_i - centre_v|.
+//
+// The basis functions are taken as polynomials p_j of the direction without their constants k_j (b_j = k_j p_j); the constants go
+// into the coefficients or into their gradients, once per splat.
+//
+// One view of 4-bit rows (the *_row kernels) is bound by memory: a thread per splat, nothing kept, codes decoded where they are
+// multiplied.  Several views, or values in another form (the *_views kernels), are bound by arithmetic: a thread works on two
+// splats at once, 128 apart, with the coefficients in registers, and all its arithmetic is on pairs, one packed single-precision
+// instruction for two results.
+typedef float2 Pair;
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ Pair operator*(float a, Pair b) { return __fmul2_rn(make_float2(a, a), b); }
+__device__ __forceinline__ Pair fma_(Pair a, Pair b, Pair c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ Pair fma_(float a, Pair b, Pair c) { return __ffma2_rn(make_float2(a, a), b, c); }
+__device__ __forceinline__ float fma_(float a, float b, float c) { return fmaf(a, b, c); }
+template <class T> __device__ __forceinline__ T all(float a);
+template <> __device__ __forceinline__ float all<float>(float a) { return a; }
+template <> __device__ __forceinline__ Pair all<Pair>(float a) { return make_float2(a, a); }
 
-__device__ __forceinline__ ViewCentre view_centre(const float* __restrict__ viewmats, int v) {
-    const float* m = viewmats + 16 * v;
-    ViewCentre c;
-#pragma unroll
-    for (int j = 0; j < 3; ++j) {
-        const double s = (double)m[j] * m[3] + (double)m[4 + j] * m[7] + (double)m[8 + j] * m[11];
-        c.hi[j] = (float)s;
-        c.lo[j] = (float)(s - (double)c.hi[j]);
-    }
-    return c;
+__device__ __forceinline__ constexpr float sh_constant(int j) {
+    constexpr float k[kNumSh] = {-0.4886025119029199f, 0.4886025119029199f, -0.4886025119029199f,
+                                 1.0925484305920792f, -1.0925484305920792f, 0.31539156525252005f, -1.0925484305920792f, 0.5462742152960396f,
+                                 -0.5900435899266435f, 2.890611442640554f, -0.4570457994644658f, 0.3731763325901154f, -0.4570457994644658f,
+                                 1.445305721320277f, -0.5900435899266435f};
+    return k[j];
 }
 
-struct Direction { float x, y, z, inv; };      // unit vector and 1 / distance
+// The difference mean - centre is what loses bits when a camera is close to a splat far from the origin, so the centre is kept as
+// a sum of two floats.
+template <class T> struct ViewCentre { T hi[3], lo[3]; };      // -centre = R^T t
 
-// The direction of a splat at the camera's own position is undefined: the bands then contribute nothing (all components 0).
-__device__ __noinline__ Direction direction_rescaled(float dx, float dy, float dz) {
-    const float m = fmaxf(fabsf(dx), fmaxf(fabsf(dy), fabsf(dz)));
-    if (dx == 0.0f && dy == 0.0f && dz == 0.0f) return {0.0f, 0.0f, 0.0f, 0.0f};
-    const int e = isfinite(m) ? ilogbf(m) : 0;
-    dx = scalbnf(dx, -e); dy = scalbnf(dy, -e); dz = scalbnf(dz, -e);
-    const float inv = rsqrtf(dx * dx + dy * dy + dz * dz);
-    return {dx * inv, dy * inv, dz * inv, scalbnf(inv, -e)};
+// Component j of R^T t.
+__device__ __forceinline__ double centre_component(const float* __restrict__ viewmats, int v, int j) {
+    const float* m = viewmats + 16 * (int64_t)v;
+    return (double)m[j] * m[3] + (double)m[4 + j] * m[7] + (double)m[8 + j] * m[11];
 }
 
-__device__ __forceinline__ Direction view_direction(const ViewCentre& c, const float mean[3]) {
-    const float dx = (mean[0] + c.hi[0]) + c.lo[0], dy = (mean[1] + c.hi[1]) + c.lo[1], dz = (mean[2] + c.hi[2]) + c.lo[2];
-    const float d2 = dx * dx + dy * dy + dz * dz;
-    if (!(d2 > 1e-30f && d2 < 1e30f)) return direction_rescaled(dx, dy, dz);
-    float inv = rsqrtf(d2);
-    inv = inv * fmaf(-0.5f * d2, inv * inv, 1.5f);
+template <class T>
+struct Directions { T x, y, z, inv; };         // unit vectors and 1 / distance
+
+// d2 leaves the caller to notice squares that left the range of floats (see eval_checked).
+template <class T>
+__device__ __forceinline__ Directions<T> view_directions(const ViewCentre<T>& c, const T mean[3], T& d2) {
+    const T dx = (mean[0] + c.hi[0]) + c.lo[0], dy = (mean[1] + c.hi[1]) + c.lo[1], dz = (mean[2] + c.hi[2]) + c.lo[2];
+    d2 = fma_(dx, dx, fma_(dy, dy, dz * dz));
+    T inv;
+    if constexpr (sizeof(T) == 8) inv = make_float2(rsqrtf(d2.x), rsqrtf(d2.y)); else inv = rsqrtf(d2);
     return {dx * inv, dy * inv, dz * inv, inv};
 }
+constexpr float kSquareMin = 1e-30f, kSquareMax = 1e30f;
 
-constexpr int kCentreChunk = 32;      // views whose centres a block keeps at a time
+template <class T>
+struct Polynomials { T p[kNumSh], t; };        // t = 5 z^2 - 1
 
-__device__ __forceinline__ void stage_centres(ViewCentre* centres_s, const float* __restrict__ viewmats, int v0, int views) {
-    const int v = v0 + threadIdx.x;
-    if (threadIdx.x < kCentreChunk && v < views) centres_s[threadIdx.x] = view_centre(viewmats, v);
+template <class T>
+__device__ __forceinline__ Polynomials<T> sh_polynomials(const Directions<T>& d) {
+    Polynomials<T> o;
+    const T x = d.x, y = d.y, z = d.z, xx = x * x, zz = z * z, nyy = (-1.0f * y) * y;
+    o.p[0] = y; o.p[1] = z; o.p[2] = x;
+    o.p[3] = x * y; o.p[4] = y * z; o.p[5] = fma_(3.0f, zz, all<T>(-1.0f)); o.p[6] = x * z; o.p[7] = xx + nyy;
+    o.t = fma_(5.0f, zz, all<T>(-1.0f));
+    o.p[8] = y * fma_(3.0f, xx, nyy); o.p[9] = o.p[3] * z; o.p[10] = y * o.t; o.p[11] = z * fma_(5.0f, zz, all<T>(-3.0f));
+    o.p[12] = x * o.t; o.p[13] = z * o.p[7]; o.p[14] = x * fma_(3.0f, nyy, xx);
+    return o;
 }
 
-// The SH values of the thread's splat: in registers from its 4-bit row, or from the block's staged span.
-template <bool ROWS>
-__device__ __forceinline__ void read_sh(float sh[kShPerSplat], const float* sh_s, const SsbShQuant& shq, int64_t i, int n_sh) {
-    if (n_sh == 0) {
+// Gradient of sum_j w_j p_j with respect to the mean: the polynomials' gradient, made tangent to the sphere, over the distance.
+template <class T>
+__device__ __forceinline__ void sh_polynomials_vjp(const Directions<T>& d, const Polynomials<T>& o, const T w[kNumSh], T v[3]) {
+    const T x = d.x, y = d.y, z = d.z, xy = o.p[3], yz = o.p[4], xz = o.p[6], c1 = o.p[7];
+    const T w7 = w[7] + w[7], w8 = 3.0f * w[8], w13 = w[13] + w[13], w14 = 3.0f * w[14], xy2 = xy + xy;
+    T gx = fma_(y, w[3], w[2]), gy = fma_(x, w[3], w[0]), gz = fma_(y, w[4], w[1]);
+    gx = fma_(z, w[6], gx); gx = fma_(x, w7, gx); gx = fma_(xy2, w8, gx); gx = fma_(yz, w[9], gx);
+    gx = fma_(o.t, w[12], gx); gx = fma_(xz, w13, gx); gx = fma_(c1, w14, gx);
+    gy = fma_(z, w[4], gy); gy = fma_(c1, w8, gy); gy = fma_(xz, w[9], gy); gy = fma_(o.t, w[10], gy);
+    gy = fma_(-1.0f, fma_(y, w7, fma_(yz, w13, xy2 * w14)), gy);
+    gz = fma_(6.0f * z, w[5], gz); gz = fma_(x, w[6], gz); gz = fma_(xy, w[9], gz);
+    gz = fma_(10.0f, fma_(yz, w[10], xz * w[12]), gz); gz = fma_(fma_(15.0f, z * z, all<T>(-3.0f)), w[11], gz); gz = fma_(c1, w[13], gz);
+    const T ndn = -1.0f * fma_(x, gx, fma_(y, gy, z * gz));
+    v[0] = fma_(x, ndn, gx) * d.inv; v[1] = fma_(y, ndn, gy) * d.inv; v[2] = fma_(z, ndn, gz) * d.inv;
+}
+
+// ---- coefficients ----
+// A code is read in place: the four bits at position 4 p of a word, or-ed into 2^23, are 2^23 + code 2^4p as a float, and the 2^-4p
+// goes into a constant; only the positions 5..7 need the word shifted first.
+__device__ __forceinline__ constexpr int code_shift(int j) { return (j & 7) > 4 ? 4 * (j & 7) - 16 : 4 * (j & 7); }
+__device__ __forceinline__ constexpr float code_unit(int j) { return 1.0f / (float)(1 << code_shift(j)); }
+__device__ __forceinline__ constexpr float code_bias(int j) { return -(8388608.0f + (float)(8 << code_shift(j))); }
+__device__ __forceinline__ float code_bits(const ShRow& r, int j, int ch) {
+    const uint32_t w = r.w[2 * ch + (j >> 3)];
+    return __uint_as_float((((j & 7) > 4 ? w >> 16 : w) & (15u << code_shift(j))) | 0x4b000000u);
+}
+// (code - 8) / code_unit(j), exact
+__device__ __forceinline__ float code_of(const ShRow& r, int j, int ch) { return code_bits(r, j, ch) + code_bias(j); }
+__device__ __forceinline__ Pair code_of(const ShRow& a, const ShRow& b, int j, int ch) {
+    return make_float2(code_bits(a, j, ch), code_bits(b, j, ch)) + all<Pair>(code_bias(j));
+}
+// A band's scale, zero above the active degree.
+__device__ __forceinline__ float active_scale(const ShRow& r, int band, int n_sh) { return n_sh > (band + 1) * (band + 1) - 1 ? sh_row_scale(r, band) : 0.0f; }
+
+// Everything about one splat by the definition, with the direction in double precision, whose range the square of a distance cannot
+// leave: for splats that are nearer to a camera than 1e-15 or farther than 1e15.  A splat at the camera's own position has no
+// direction: the bands contribute nothing.  Forward (v_out NULL): the values of all views at out.  Backward: g receives the
+// gradients of the mean (3), of DC (3) and of the coefficients (45).
+__device__ __noinline__ void eval_checked(const SsbSplats sp, const float* sh, const void* rows, int64_t i, int64_t n, int views,
+                                          const float* viewmats, int n_sh, float* out, const float* v_out, float* g) {
+    float W[kShPerSplat];
+    if (rows) decode_sh_row(load_sh_row(rows, i), W);
+    else for (int k = 0; k < 3 * n_sh; ++k) W[k] = sh[k];
+    if (v_out) for (int k = 0; k < 6 + kShPerSplat; ++k) g[k] = 0.0f;
+    for (int v = 0; v < views; ++v) {
+        double d[3], r2 = 0.0;
+        for (int k = 0; k < 3; ++k) { d[k] = (double)sp.means[3 * i + k] + centre_component(viewmats, v, k); r2 += d[k] * d[k]; }
+        const double inv = r2 == 0.0 ? 0.0 : 1.0 / sqrt(r2);
+        const Directions<float> dir = {(float)(d[0] * inv), (float)(d[1] * inv), (float)(d[2] * inv), (float)inv};
+        Polynomials<float> o = sh_polynomials(dir);
+        if (r2 == 0.0) o.p[5] = 0.0f;
+        if (!v_out) {
+            for (int ch = 0; ch < 3; ++ch) {
+                float c = sp.features_dc ? kShC0 * sp.features_dc[3 * i + ch] : 0.0f;
+                for (int j = 0; j < n_sh; ++j) c += o.p[j] * sh_constant(j) * W[3 * j + ch];
+                out[3 * ((int64_t)v * n + i) + ch] = c;
+            }
+        } else {
+            const float* go = v_out + 3 * ((int64_t)v * n + i);
+            float w[kNumSh] = {}, vm[3];
+            for (int ch = 0; ch < 3; ++ch) {
+                g[3 + ch] += kShC0 * go[ch];
+                for (int j = 0; j < n_sh; ++j) {
+                    w[j] += sh_constant(j) * W[3 * j + ch] * go[ch];
+                    g[6 + 3 * j + ch] += o.p[j] * sh_constant(j) * go[ch];
+                }
+            }
+            sh_polynomials_vjp(dir, o, w, vm);
+            for (int k = 0; k < 3; ++k) g[k] += vm[k];
+        }
+    }
+}
+
+// ---- one view of 4-bit rows ----
+constexpr int kRowBlock = 128;
+
+// Components of -centre of view 0 as two floats each, by the block's first three threads; a barrier follows.
+__device__ __forceinline__ void stage_centre(ViewCentre<float>& c, const float* __restrict__ viewmats) {
+    if (threadIdx.x < 3) {
+        const double s = centre_component(viewmats, 0, threadIdx.x);
+        c.hi[threadIdx.x] = (float)s;
+        c.lo[threadIdx.x] = (float)(s - (double)(float)s);
+    }
+}
+
+__global__ void __launch_bounds__(kRowBlock) sh_eval_fwd_row_kernel(SsbSplats sp, const void* __restrict__ rows, int64_t n, const float* __restrict__ viewmats,
+                                                                    int n_sh, float* __restrict__ out) {
+    __shared__ ViewCentre<float> centre_s;
+    const int64_t i = (int64_t)blockIdx.x * kRowBlock + threadIdx.x, il = min(i, n - 1);
+    ShRow r = {};
+    if (n_sh > 0) r = load_sh_row(rows, il);
+    const float mean[3] = {sp.means[3 * il], sp.means[3 * il + 1], sp.means[3 * il + 2]};
+    float c[3] = {0.f, 0.f, 0.f};
+    if (sp.features_dc) { c[0] = sp.features_dc[3 * il]; c[1] = sp.features_dc[3 * il + 1]; c[2] = sp.features_dc[3 * il + 2]; }
+    stage_centre(centre_s, viewmats);
+    __syncthreads();
+    if (i >= n) return;
+    float d2;
+    const Polynomials<float> o = sh_polynomials(view_directions(centre_s, mean, d2));
 #pragma unroll
-        for (int k = 0; k < kShPerSplat; ++k) sh[k] = 0.0f;
-    } else if (ROWS) {
-        decode_sh_row(load_sh_row(shq.packed, i), sh);
+    for (int ch = 0; ch < 3; ++ch) c[ch] *= kShC0;
+#pragma unroll
+    for (int b = 0; b < 3; ++b) {
+        float t[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < kNumSh; ++j)
+            if (sh_band(j) == b) {
+                const float f = (sh_constant(j) * code_unit(j)) * o.p[j];
+#pragma unroll
+                for (int ch = 0; ch < 3; ++ch) t[ch] = fmaf(f, code_of(r, j, ch), t[ch]);
+            }
+        const float s = active_scale(r, b, n_sh);
+#pragma unroll
+        for (int ch = 0; ch < 3; ++ch) c[ch] = fmaf(s, t[ch], c[ch]);
+    }
+    out[3 * i] = c[0]; out[3 * i + 1] = c[1]; out[3 * i + 2] = c[2];
+    if (!(d2 > kSquareMin && d2 < kSquareMax)) eval_checked(sp, nullptr, n_sh ? rows : nullptr, i, n, 1, viewmats, n_sh, out, nullptr, nullptr);
+}
+
+__global__ void __launch_bounds__(kRowBlock) sh_eval_bwd_row_kernel(SsbSplats sp, const void* __restrict__ rows, int64_t n, const float* __restrict__ viewmats,
+                                                                    int n_sh, const float* __restrict__ v_out, SsbSplats gr, int accumulate) {
+    __shared__ __align__(16) float sh_s[kRowBlock * kShPerSplat];
+    __shared__ __align__(16) float mean_s[kRowBlock * 3];
+    __shared__ __align__(16) float dc_s[kRowBlock * 3];
+    __shared__ ViewCentre<float> centre_s;
+    const int64_t first = (int64_t)blockIdx.x * kRowBlock, i = first + threadIdx.x, il = min(i, n - 1);
+    ShRow r = {};
+    if (n_sh > 0) r = load_sh_row(rows, il);
+    const float mean[3] = {sp.means[3 * il], sp.means[3 * il + 1], sp.means[3 * il + 2]};
+    const float g[3] = {v_out[3 * il], v_out[3 * il + 1], v_out[3 * il + 2]};
+    stage_centre(centre_s, viewmats);
+    __syncthreads();
+    float d2, w[kNumSh], vm[3];
+    const Directions<float> d = view_directions(centre_s, mean, d2);
+    const Polynomials<float> o = sh_polynomials(d);
+#pragma unroll
+    for (int j = 0; j < kNumSh; ++j) {
+        float t = code_of(r, j, 0) * g[0];
+        t = fmaf(code_of(r, j, 1), g[1], t);
+        t = fmaf(code_of(r, j, 2), g[2], t);
+        const bool active = n_sh > (sh_band(j) + 1) * (sh_band(j) + 1) - 1;
+        w[j] = active ? ((sh_constant(j) * code_unit(j)) * sh_row_scale(r, sh_band(j))) * t : 0.0f;
+#pragma unroll
+        for (int ch = 0; ch < 3; ++ch) sh_s[threadIdx.x * kShPerSplat + 3 * j + ch] = active ? sh_constant(j) * o.p[j] * g[ch] : 0.0f;
+    }
+    sh_polynomials_vjp(d, o, w, vm);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) { mean_s[3 * threadIdx.x + k] = vm[k]; dc_s[3 * threadIdx.x + k] = kShC0 * g[k]; }
+    if (!(d2 > kSquareMin && d2 < kSquareMax)) {
+        float e[6 + kShPerSplat];
+        eval_checked(sp, nullptr, n_sh ? rows : nullptr, il, n, 1, viewmats, n_sh, nullptr, v_out, e);
+        for (int k = 0; k < 3; ++k) { mean_s[3 * threadIdx.x + k] = e[k]; dc_s[3 * threadIdx.x + k] = e[3 + k]; }
+        for (int k = 0; k < kShPerSplat; ++k) sh_s[threadIdx.x * kShPerSplat + k] = e[6 + k];
+    }
+    span_written();
+    __syncthreads();
+    const int count = (int)min((int64_t)kRowBlock, n - first);
+    if (gr.features_sh) store_span(gr.features_sh + kShPerSplat * first, sh_s, kShPerSplat * count, kShPerSplat * kRowBlock, accumulate != 0);
+    if (gr.means) store_span(gr.means + 3 * first, mean_s, 3 * count, 3 * kRowBlock, accumulate != 0);
+    if (gr.features_dc) store_span(gr.features_dc + 3 * first, dc_s, 3 * count, 3 * kRowBlock, accumulate != 0);
+    bulk_done();
+}
+
+// ---- several views, or values in another form ----
+constexpr int kEvalTile = 2 * kProjBlock;      // splats per block and step
+constexpr int kCentreChunk = 32;               // views whose centres a block keeps at a time
+constexpr int kEvalShBytes = kEvalTile * kShPerSplat * (int)sizeof(float);
+
+__device__ __forceinline__ void stage_centres(ViewCentre<Pair>* centres_s, const float* __restrict__ viewmats, int v0, int views) {
+    const int v = threadIdx.x / 3, j = threadIdx.x - 3 * v;
+    if (v < kCentreChunk && v0 + v < views) {
+        const double s = centre_component(viewmats, v0 + v, j);
+        centres_s[v].hi[j] = all<Pair>((float)s);
+        centres_s[v].lo[j] = all<Pair>((float)(s - (double)(float)s));
+    }
+}
+static_assert(3 * kCentreChunk <= kProjBlock, "one thread per component of a chunk's centres");
+
+__device__ __forceinline__ void stage_tile(float* sh_s, unsigned char* raw_s, const SsbSplats& sp, const SsbShQuant& shq, int64_t first, int64_t n) {
+    stage_sh(sh_s, raw_s, sp.features_sh, shq.packed, shq.bounds, shq.bits, shq.bounds_stride, first, n);
+    __syncthreads();
+    stage_sh(sh_s + kProjBlock * kShPerSplat, raw_s, sp.features_sh, shq.packed, shq.bounds, shq.bits, shq.bounds_stride, first + kProjBlock, n);
+    __syncthreads();
+}
+
+// k_j W[j][ch] of both splats, zero above the active degree.
+template <bool ROWS>
+__device__ __forceinline__ void read_coefficients(Pair W[kShPerSplat], const float* sh_s, const void* rows, int64_t i0, int64_t i1, int n_sh) {
+    if (ROWS) {
+        ShRow a = {}, b = {};
+        if (n_sh > 0) { a = load_sh_row(rows, i0); b = load_sh_row(rows, i1); }
+#pragma unroll
+        for (int j = 0; j < kNumSh; ++j) {
+            const Pair f = (sh_constant(j) * code_unit(j)) * make_float2(active_scale(a, sh_band(j), n_sh), active_scale(b, sh_band(j), n_sh));
+#pragma unroll
+            for (int ch = 0; ch < 3; ++ch) W[3 * j + ch] = f * code_of(a, b, j, ch);
+        }
     } else {
 #pragma unroll
-        for (int k = 0; k < kShPerSplat; ++k) sh[k] = sh_s[threadIdx.x * kShPerSplat + k];
+        for (int j = 0; j < kNumSh; ++j)
+#pragma unroll
+            for (int ch = 0; ch < 3; ++ch) {
+                const int k = 3 * j + ch;
+                W[k] = j < n_sh ? sh_constant(j) * make_float2(sh_s[threadIdx.x * kShPerSplat + k], sh_s[(threadIdx.x + kProjBlock) * kShPerSplat + k])
+                                : all<Pair>(0.0f);
+            }
     }
 }
 
+__device__ __forceinline__ void load_pairs(const float* __restrict__ p, int64_t i0, int64_t i1, Pair v[3]) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) v[k] = make_float2(p[3 * i0 + k], p[3 * i1 + k]);
+}
+
+constexpr int kFwdBlocksPerSm = 3, kBwdBlocksPerSm = 2;       // what their registers allow; the grids are this many blocks
+
 template <bool ROWS>
-__global__ void __launch_bounds__(kProjBlock) sh_eval_fwd_kernel(SsbSplats sp, SsbShQuant shq, int64_t n, int views, const float* __restrict__ viewmats,
-                                                                 int n_sh, float* __restrict__ out) {
-    __shared__ __align__(16) float sh_s[ROWS ? 4 : kProjBlock * kShPerSplat];
-    __shared__ __align__(16) unsigned char raw_s[ROWS ? 16 : kShRawBytes];
-    __shared__ ViewCentre centres_s[kCentreChunk];
+__global__ void __launch_bounds__(kProjBlock, kFwdBlocksPerSm) sh_eval_fwd_views_kernel(SsbSplats sp, SsbShQuant shq, int64_t n, int views,
+                                                                                        const float* __restrict__ viewmats, int n_sh,
+                                                                                        float* __restrict__ out) {
+    extern __shared__ __align__(16) unsigned char dyn_s[];
+    __shared__ ViewCentre<Pair> centres_s[kCentreChunk];
+    float* sh_s = (float*)dyn_s;
     stage_centres(centres_s, viewmats, 0, views);
     __syncthreads();
-    for (int64_t first = (int64_t)blockIdx.x * kProjBlock; first < n; first += (int64_t)gridDim.x * kProjBlock) {
-        const int64_t i = first + threadIdx.x;
-        if (!ROWS && n_sh > 0) {
+    for (int64_t first = (int64_t)blockIdx.x * kEvalTile; first < n; first += (int64_t)gridDim.x * kEvalTile) {
+        const int64_t i0 = first + threadIdx.x, i1 = i0 + kProjBlock, l0 = min(i0, n - 1), l1 = min(i1, n - 1);
+        if (!ROWS) {
             __syncthreads();
-            stage_sh(sh_s, raw_s, sp.features_sh, shq.packed, shq.bounds, shq.bits, shq.bounds_stride, first, n);
-            __syncthreads();
+            stage_tile(sh_s, dyn_s + kEvalShBytes, sp, shq, first, n);
         }
-        const int64_t il = min(i, n - 1);
-        const float mean[3] = {sp.means[3 * il], sp.means[3 * il + 1], sp.means[3 * il + 2]};
-        float dc[3] = {0.f, 0.f, 0.f};
-        if (sp.features_dc)
+        Pair mean[3], dc[3] = {all<Pair>(0.f), all<Pair>(0.f), all<Pair>(0.f)}, W[kShPerSplat];
+        load_pairs(sp.means, l0, l1, mean);
+        if (sp.features_dc) {
+            load_pairs(sp.features_dc, l0, l1, dc);
 #pragma unroll
-            for (int ch = 0; ch < 3; ++ch) dc[ch] = kShC0 * sp.features_dc[3 * il + ch];
-        float sh[kShPerSplat];
-        read_sh<ROWS>(sh, sh_s, shq, il, n_sh);
+            for (int ch = 0; ch < 3; ++ch) dc[ch] = kShC0 * dc[ch];
+        }
+        read_coefficients<ROWS>(W, sh_s, shq.packed, l0, l1, n_sh);
+        float least = kSquareMax, most = kSquareMin;
         for (int v0 = 0; v0 < views; v0 += kCentreChunk) {
             if (views > kCentreChunk) {
                 __syncthreads();
@@ -230,47 +456,73 @@ __global__ void __launch_bounds__(kProjBlock) sh_eval_fwd_kernel(SsbSplats sp, S
                 __syncthreads();
             }
             const int v1 = min(views - v0, kCentreChunk);
-            for (int v = 0; v < v1; ++v) {
-                const Direction d = view_direction(centres_s[v], mean);
-                float b[kNumSh];
-                sh_basis(d.x, d.y, d.z, b);
-                if (d.inv == 0.0f) b[5] = 0.0f;            // no direction: the one basis function that does not vanish by itself
-                float c[3] = {dc[0], dc[1], dc[2]};
+            float* o0 = out + 3 * ((int64_t)v0 * n + i0);
+            for (int v = 0; v < v1; ++v, o0 += 3 * n) {
+                Pair d2, c[3] = {dc[0], dc[1], dc[2]};
+                const Polynomials<Pair> o = sh_polynomials(view_directions(centres_s[v], mean, d2));
+                least = fminf(least, fminf(d2.x, d2.y)); most = fmaxf(most, fmaxf(d2.x, d2.y));
 #pragma unroll
                 for (int j = 0; j < kNumSh; ++j)
-                    if (j < n_sh)
 #pragma unroll
-                        for (int ch = 0; ch < 3; ++ch) c[ch] += b[j] * sh[3 * j + ch];
-                if (i < n) {
-                    float* o = out + 3 * ((int64_t)(v0 + v) * n + i);
-                    o[0] = c[0]; o[1] = c[1]; o[2] = c[2];
+                    for (int ch = 0; ch < 3; ++ch) c[ch] = fma_(o.p[j], W[3 * j + ch], c[ch]);
+#pragma unroll
+                for (int ch = 0; ch < 3; ++ch) {
+                    if (i0 < n) o0[ch] = c[ch].x;
+                    if (i1 < n) o0[3 * kProjBlock + ch] = c[ch].y;
                 }
             }
+        }
+        if (!(least > kSquareMin && most < kSquareMax)) {
+            const void* rows = ROWS && n_sh > 0 ? shq.packed : nullptr;
+            if (i0 < n) eval_checked(sp, sh_s + threadIdx.x * kShPerSplat, rows, i0, n, views, viewmats, n_sh, out, nullptr, nullptr);
+            if (i1 < n) eval_checked(sp, sh_s + (threadIdx.x + kProjBlock) * kShPerSplat, rows, i1, n, views, viewmats, n_sh, out, nullptr, nullptr);
         }
     }
 }
 
-template <bool ROWS>
-__global__ void __launch_bounds__(kProjBlock) sh_eval_bwd_kernel(SsbSplats sp, SsbShQuant shq, int64_t n, int views, const float* __restrict__ viewmats,
-                                                                 int n_sh, const float* __restrict__ v_out, SsbSplats gr, int accumulate) {
-    __shared__ __align__(16) float sh_s[kProjBlock * kShPerSplat];       // values on the way in, their gradients on the way out
-    __shared__ __align__(16) float mean_s[kProjBlock * 3];
-    __shared__ __align__(16) float dc_s[kProjBlock * 3];
-    __shared__ __align__(16) unsigned char raw_s[ROWS ? 16 : kShRawBytes];
-    __shared__ ViewCentre centres_s[kCentreChunk];
-    stage_centres(centres_s, viewmats, 0, views);
-    for (int64_t first = (int64_t)blockIdx.x * kProjBlock; first < n; first += (int64_t)gridDim.x * kProjBlock) {
-        const int64_t i = first + threadIdx.x, il = min(i, n - 1);
-        __syncthreads();
-        if (!ROWS && n_sh > 0) {
-            stage_sh(sh_s, raw_s, sp.features_sh, shq.packed, shq.bounds, shq.bits, shq.bounds_stride, first, n);
-            __syncthreads();
-        }
-        const float mean[3] = {sp.means[3 * il], sp.means[3 * il + 1], sp.means[3 * il + 2]};
-        float sh[kShPerSplat], g_mean[3] = {0.f, 0.f, 0.f}, g_dc[3] = {0.f, 0.f, 0.f}, g_sh[kShPerSplat];
-        read_sh<ROWS>(sh, sh_s, shq, il, n_sh);
+// The gradients of the next views travel to shared memory while a view is worked on: each thread copies and reads its own six
+// numbers, so no barrier is needed.
+constexpr int kGradAhead = 3;
+struct GradRing { float g[kGradAhead + 1][3][kEvalTile]; };
+__device__ __forceinline__ void fetch_grads(GradRing& ring, const float* __restrict__ v_out, int64_t n, int v, int views, int64_t l0, int64_t l1) {
+    if (v < views) {
+        const float* p = v_out + 3 * (int64_t)v * n;
+        float* q = &ring.g[v & kGradAhead][0][threadIdx.x];
+        const uint32_t s = (uint32_t)__cvta_generic_to_shared(q);
 #pragma unroll
-        for (int k = 0; k < kShPerSplat; ++k) g_sh[k] = 0.f;
+        for (int k = 0; k < 3; ++k) {
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s + 4 * kEvalTile * k), "l"(p + 3 * l0 + k) : "memory");
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s + 4 * kEvalTile * k + 4 * kProjBlock), "l"(p + 3 * l1 + k) : "memory");
+        }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+
+template <bool ROWS>
+__global__ void __launch_bounds__(kProjBlock, kBwdBlocksPerSm) sh_eval_bwd_views_kernel(SsbSplats sp, SsbShQuant shq, int64_t n, int views,
+                                                                                        const float* __restrict__ viewmats, int n_sh,
+                                                                                        const float* __restrict__ v_out, SsbSplats gr, int accumulate) {
+    extern __shared__ __align__(16) unsigned char dyn_s[];
+    __shared__ __align__(16) float mean_s[kEvalTile * 3];
+    __shared__ __align__(16) float dc_s[kEvalTile * 3];
+    __shared__ GradRing ring;
+    __shared__ ViewCentre<Pair> centres_s[kCentreChunk];
+    float* sh_s = (float*)dyn_s;                 // values on the way in, their gradients on the way out
+    stage_centres(centres_s, viewmats, 0, views);
+    for (int64_t first = (int64_t)blockIdx.x * kEvalTile; first < n; first += (int64_t)gridDim.x * kEvalTile) {
+        const int64_t i0 = first + threadIdx.x, i1 = i0 + kProjBlock, l0 = min(i0, n - 1), l1 = min(i1, n - 1);
+        __syncthreads();
+        if (!ROWS) stage_tile(sh_s, dyn_s + kEvalShBytes, sp, shq, first, n);
+#pragma unroll
+        for (int v = 0; v < kGradAhead; ++v) fetch_grads(ring, v_out, n, v, views, l0, l1);
+        Pair mean[3], g_mean[3], g_dc[3], g_sh[kShPerSplat], W[kShPerSplat];
+        load_pairs(sp.means, l0, l1, mean);
+        read_coefficients<ROWS>(W, sh_s, shq.packed, l0, l1, n_sh);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) g_mean[k] = g_dc[k] = all<Pair>(0.f);
+#pragma unroll
+        for (int k = 0; k < kShPerSplat; ++k) g_sh[k] = all<Pair>(0.f);
+        float least = kSquareMax, most = kSquareMin;
         for (int v0 = 0; v0 < views; v0 += kCentreChunk) {
             if (views > kCentreChunk) {
                 __syncthreads();
@@ -279,42 +531,61 @@ __global__ void __launch_bounds__(kProjBlock) sh_eval_bwd_kernel(SsbSplats sp, S
             }
             const int v1 = min(views - v0, kCentreChunk);
             for (int v = 0; v < v1; ++v) {
-                const float* gp = v_out + 3 * ((int64_t)(v0 + v) * n + il);
-                const float g[3] = {gp[0], gp[1], gp[2]};
-                const Direction d = view_direction(centres_s[v], mean);
-                float b[kNumSh], w[kNumSh];
-                sh_basis(d.x, d.y, d.z, b);
-                if (d.inv == 0.0f) b[5] = 0.0f;
+                Pair d2, g[3], w[kNumSh], vm[3];
+                fetch_grads(ring, v_out, n, v0 + v + kGradAhead, views, l0, l1);
+                asm volatile("cp.async.wait_group %0;" ::"n"(kGradAhead) : "memory");
+#pragma unroll
+                for (int k = 0; k < 3; ++k)
+                    g[k] = make_float2(ring.g[(v0 + v) & kGradAhead][k][threadIdx.x], ring.g[(v0 + v) & kGradAhead][k][threadIdx.x + kProjBlock]);
+                const Directions<Pair> d = view_directions(centres_s[v], mean, d2);
+                const Polynomials<Pair> o = sh_polynomials(d);
+                least = fminf(least, fminf(d2.x, d2.y)); most = fmaxf(most, fmaxf(d2.x, d2.y));
 #pragma unroll
                 for (int j = 0; j < kNumSh; ++j) {
-                    w[j] = 0.0f;
-                    if (j < n_sh) {
+                    w[j] = W[3 * j] * g[0];
+                    w[j] = fma_(W[3 * j + 1], g[1], w[j]);
+                    w[j] = fma_(W[3 * j + 2], g[2], w[j]);
 #pragma unroll
-                        for (int ch = 0; ch < 3; ++ch) { w[j] += sh[3 * j + ch] * g[ch]; g_sh[3 * j + ch] += b[j] * g[ch]; }
-                    }
+                    for (int ch = 0; ch < 3; ++ch) g_sh[3 * j + ch] = fma_(o.p[j], g[ch], g_sh[3 * j + ch]);
                 }
+                sh_polynomials_vjp(d, o, w, vm);
 #pragma unroll
-                for (int ch = 0; ch < 3; ++ch) g_dc[ch] += kShC0 * g[ch];
-                float vn[3];
-                sh_basis_vjp(d.x, d.y, d.z, w, vn);
-                const float dn = d.x * vn[0] + d.y * vn[1] + d.z * vn[2];
-                g_mean[0] += (vn[0] - d.x * dn) * d.inv;
-                g_mean[1] += (vn[1] - d.y * dn) * d.inv;
-                g_mean[2] += (vn[2] - d.z * dn) * d.inv;
+                for (int k = 0; k < 3; ++k) { g_dc[k] = fma_(kShC0, g[k], g_dc[k]); g_mean[k] = g_mean[k] + vm[k]; }
             }
+        }
+        float e0[6 + kShPerSplat], e1[6 + kShPerSplat];
+        const bool checked = !(least > kSquareMin && most < kSquareMax);
+        if (checked) {
+            const void* rows = ROWS && n_sh > 0 ? shq.packed : nullptr;
+            eval_checked(sp, sh_s + threadIdx.x * kShPerSplat, rows, l0, n, views, viewmats, n_sh, nullptr, v_out, e0);
+            // the second splat's values exist only inside the array
+            if (i1 < n) eval_checked(sp, sh_s + (threadIdx.x + kProjBlock) * kShPerSplat, rows, l1, n, views, viewmats, n_sh, nullptr, v_out, e1);
         }
         bulk_done();
         __syncthreads();          // the previous tile's copies have left, and every thread has read its values
+        const int t0 = threadIdx.x, t1 = threadIdx.x + kProjBlock;
 #pragma unroll
-        for (int k = 0; k < 3; ++k) { mean_s[3 * threadIdx.x + k] = g_mean[k]; dc_s[3 * threadIdx.x + k] = g_dc[k]; }
+        for (int k = 0; k < 3; ++k) {
+            mean_s[3 * t0 + k] = g_mean[k].x; mean_s[3 * t1 + k] = g_mean[k].y;
+            dc_s[3 * t0 + k] = g_dc[k].x; dc_s[3 * t1 + k] = g_dc[k].y;
+        }
 #pragma unroll
-        for (int k = 0; k < kShPerSplat; ++k) sh_s[kShPerSplat * threadIdx.x + k] = g_sh[k];
+        for (int j = 0; j < kNumSh; ++j)
+#pragma unroll
+            for (int ch = 0; ch < 3; ++ch) {
+                const Pair t = j < n_sh ? sh_constant(j) * g_sh[3 * j + ch] : all<Pair>(0.0f);
+                sh_s[kShPerSplat * t0 + 3 * j + ch] = t.x; sh_s[kShPerSplat * t1 + 3 * j + ch] = t.y;
+            }
+        if (checked) {
+            for (int k = 0; k < 3; ++k) { mean_s[3 * t0 + k] = e0[k]; mean_s[3 * t1 + k] = e1[k]; dc_s[3 * t0 + k] = e0[3 + k]; dc_s[3 * t1 + k] = e1[3 + k]; }
+            for (int k = 0; k < kShPerSplat; ++k) { sh_s[kShPerSplat * t0 + k] = e0[6 + k]; sh_s[kShPerSplat * t1 + k] = e1[6 + k]; }
+        }
         span_written();
         __syncthreads();
-        const int count = (int)min((int64_t)kProjBlock, n - first);
-        if (gr.means) store_span(gr.means + 3 * first, mean_s, 3 * count, 3 * kProjBlock, accumulate != 0);
-        if (gr.features_dc) store_span(gr.features_dc + 3 * first, dc_s, 3 * count, 3 * kProjBlock, accumulate != 0);
-        if (gr.features_sh) store_span(gr.features_sh + kShPerSplat * first, sh_s, kShPerSplat * count, kProjBlock * kShPerSplat, accumulate != 0);
+        const int count = (int)min((int64_t)kEvalTile, n - first);
+        if (gr.means) store_span(gr.means + 3 * first, mean_s, 3 * count, 3 * kEvalTile, accumulate != 0);
+        if (gr.features_dc) store_span(gr.features_dc + 3 * first, dc_s, 3 * count, 3 * kEvalTile, accumulate != 0);
+        if (gr.features_sh) store_span(gr.features_sh + kShPerSplat * first, sh_s, kShPerSplat * count, kShPerSplat * kEvalTile, accumulate != 0);
         if (!ROWS) bulk_done();   // the next tile is staged into the same span
     }
     bulk_done();
@@ -347,9 +618,19 @@ int ssb_sh_eval_fwd(const SsbSplats* splats, const SsbShQuant* shq, int64_t n, c
     if (int e = check_eval(splats, shq, n, cams, "ssb_sh_eval_fwd", &q, &n_sh)) return e;
     if (n == 0 || cams->count == 0) return SSB_OK;
     SSB_REQUIRE(d_values && ((uintptr_t)d_values & 3) == 0, "ssb_sh_eval_fwd: d_values is NULL or not on a 4-byte boundary");
-    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(n, kProjBlock), 148 * 8);
-    if (q.bits == 4) sh_eval_fwd_kernel<true><<<blocks, kProjBlock, 0, (cudaStream_t)stream>>>(*splats, q, n, cams->count, cams->d_viewmats, n_sh, d_values);
-    else sh_eval_fwd_kernel<false><<<blocks, kProjBlock, 0, (cudaStream_t)stream>>>(*splats, q, n, cams->count, cams->d_viewmats, n_sh, d_values);
+    cudaStream_t st = (cudaStream_t)stream;
+    const bool rows = q.bits == 4 || n_sh == 0;
+    if (rows && cams->count == 1) {
+        sh_eval_fwd_row_kernel<<<(unsigned)ceil_div(n, kRowBlock), kRowBlock, 0, st>>>(*splats, q.packed, n, cams->d_viewmats, n_sh, d_values);
+    } else {
+        const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(n, kEvalTile), 148 * kFwdBlocksPerSm);
+        constexpr int smem = kEvalShBytes + kShRawBytes;
+        if (rows) sh_eval_fwd_views_kernel<true><<<blocks, kProjBlock, 0, st>>>(*splats, q, n, cams->count, cams->d_viewmats, n_sh, d_values);
+        else {
+            if (int e = ensure_dynamic_smem((const void*)sh_eval_fwd_views_kernel<false>, smem)) return e;
+            sh_eval_fwd_views_kernel<false><<<blocks, kProjBlock, smem, st>>>(*splats, q, n, cams->count, cams->d_viewmats, n_sh, d_values);
+        }
+    }
     SSB_LAUNCHED("sh_eval_fwd_kernel");
     return SSB_OK;
 }
@@ -365,9 +646,18 @@ int ssb_sh_eval_bwd(const SsbSplats* splats, const SsbShQuant* shq, int64_t n, c
     SSB_REQUIRE(d_v_values || cams->count == 0, "ssb_sh_eval_bwd: NULL argument");
     SSB_REQUIRE((((uintptr_t)d_v_values | (uintptr_t)grads->means | (uintptr_t)grads->features_dc | (uintptr_t)grads->features_sh) & 3) == 0,
                 "ssb_sh_eval_bwd: arrays must lie on 4-byte boundaries");
-    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(n, kProjBlock), 148 * 8);
-    if (q.bits == 4) sh_eval_bwd_kernel<true><<<blocks, kProjBlock, 0, (cudaStream_t)stream>>>(*splats, q, n, cams->count, cams->d_viewmats, n_sh, d_v_values, *grads, accumulate);
-    else sh_eval_bwd_kernel<false><<<blocks, kProjBlock, 0, (cudaStream_t)stream>>>(*splats, q, n, cams->count, cams->d_viewmats, n_sh, d_v_values, *grads, accumulate);
+    cudaStream_t st = (cudaStream_t)stream;
+    const bool rows = q.bits == 4 || n_sh == 0;
+    if (rows && cams->count == 1) {
+        sh_eval_bwd_row_kernel<<<(unsigned)ceil_div(n, kRowBlock), kRowBlock, 0, st>>>(*splats, q.packed, n, cams->d_viewmats, n_sh, d_v_values, *grads, accumulate);
+    } else {
+        const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(n, kEvalTile), 148 * kBwdBlocksPerSm);
+        const void* kernel = rows ? (const void*)sh_eval_bwd_views_kernel<true> : (const void*)sh_eval_bwd_views_kernel<false>;
+        const int smem = kEvalShBytes + (rows ? 0 : kShRawBytes);
+        if (int e = ensure_dynamic_smem(kernel, smem)) return e;
+        if (rows) sh_eval_bwd_views_kernel<true><<<blocks, kProjBlock, smem, st>>>(*splats, q, n, cams->count, cams->d_viewmats, n_sh, d_v_values, *grads, accumulate);
+        else sh_eval_bwd_views_kernel<false><<<blocks, kProjBlock, smem, st>>>(*splats, q, n, cams->count, cams->d_viewmats, n_sh, d_v_values, *grads, accumulate);
+    }
     SSB_LAUNCHED("sh_eval_bwd_kernel");
     return SSB_OK;
 }
