@@ -162,11 +162,24 @@ template <class T> __device__ __forceinline__ T all(float a);
 template <> __device__ __forceinline__ float all<float>(float a) { return a; }
 template <> __device__ __forceinline__ Pair all<Pair>(float a) { return make_float2(a, a); }
 
+// b_j = sh_constant(j) p_j.  The polynomials are scaled so that none of them, nor a component of a gradient, needs a constant
+// factor (a constant costs a packed instruction two registers or two moves):
+//   y, z, x | 2xy, 2yz, z^2 - 1/3, 2xz, x^2 - y^2 | y(3x^2 - y^2), 2xyz, y(z^2 - 1/5), z(z^2 - 3/5), x(z^2 - 1/5), z(x^2 - y^2),
+//   x(x^2 - 3y^2)
 __device__ __forceinline__ constexpr float sh_constant(int j) {
     constexpr float k[kNumSh] = {-0.4886025119029199f, 0.4886025119029199f, -0.4886025119029199f,
-                                 1.0925484305920792f, -1.0925484305920792f, 0.31539156525252005f, -1.0925484305920792f, 0.5462742152960396f,
-                                 -0.5900435899266435f, 2.890611442640554f, -0.4570457994644658f, 0.3731763325901154f, -0.4570457994644658f,
+                                 0.5462742152960396f, -0.5462742152960396f, 0.94617469575756f, -0.5462742152960396f, 0.5462742152960396f,
+                                 -0.5900435899266435f, 1.445305721320277f, -2.285228997322329f, 1.865881662950577f, -2.285228997322329f,
                                  1.445305721320277f, -0.5900435899266435f};
+    return k[j];
+}
+// What coefficient j is multiplied by in the sums w_j that sh_polynomials_vjp takes: b_j's constant times the constant that its
+// gradient's components share.
+__device__ __forceinline__ constexpr float sh_grad_constant(int j) {
+    constexpr float k[kNumSh] = {-0.4886025119029199f, 0.4886025119029199f, -0.4886025119029199f,
+                                 1.0925484305920792f, -1.0925484305920792f, 1.89234939151512f, -1.0925484305920792f, 1.0925484305920792f,
+                                 -1.7701307697799304f, 1.445305721320277f, -2.285228997322329f, 5.597644988851731f, -2.285228997322329f,
+                                 1.445305721320277f, -1.7701307697799304f};
     return k[j];
 }
 
@@ -195,34 +208,34 @@ __device__ __forceinline__ Directions<T> view_directions(const ViewCentre<T>& c,
 constexpr float kSquareMin = 1e-30f, kSquareMax = 1e30f;
 
 template <class T>
-struct Polynomials { T p[kNumSh], t; };        // t = 5 z^2 - 1
+struct Polynomials { T p[kNumSh], ny, x2, t; };        // -y, 2x, z^2 - 1/5
 
 template <class T>
 __device__ __forceinline__ Polynomials<T> sh_polynomials(const Directions<T>& d) {
     Polynomials<T> o;
-    const T x = d.x, y = d.y, z = d.z, xx = x * x, zz = z * z, nyy = (-1.0f * y) * y;
+    const T x = d.x, y = d.y, z = d.z, zz = z * z, y2 = y + y;
+    o.ny = -1.0f * y; o.x2 = x + x; o.t = zz + all<T>(-0.2f);
     o.p[0] = y; o.p[1] = z; o.p[2] = x;
-    o.p[3] = x * y; o.p[4] = y * z; o.p[5] = fma_(3.0f, zz, all<T>(-1.0f)); o.p[6] = x * z; o.p[7] = xx + nyy;
-    o.t = fma_(5.0f, zz, all<T>(-1.0f));
-    o.p[8] = y * fma_(3.0f, xx, nyy); o.p[9] = o.p[3] * z; o.p[10] = y * o.t; o.p[11] = z * fma_(5.0f, zz, all<T>(-3.0f));
-    o.p[12] = x * o.t; o.p[13] = z * o.p[7]; o.p[14] = x * fma_(3.0f, nyy, xx);
+    o.p[3] = o.x2 * y; o.p[4] = y2 * z; o.p[5] = zz + all<T>(-1.0f / 3.0f); o.p[6] = o.x2 * z; o.p[7] = fma_(x, x, o.ny * y);
+    o.p[8] = y * fma_(o.x2, x, o.p[7]); o.p[9] = o.p[3] * z; o.p[10] = y * o.t; o.p[11] = z * (zz + all<T>(-0.6f));
+    o.p[12] = x * o.t; o.p[13] = z * o.p[7]; o.p[14] = x * fma_(y2, o.ny, o.p[7]);
     return o;
 }
 
-// Gradient of sum_j w_j p_j with respect to the mean: the polynomials' gradient, made tangent to the sphere, over the distance.
+// Gradient with respect to the mean of sum_j b_j W_j, given w_j = sh_grad_constant(j) W_j: the polynomials' gradient, made tangent
+// to the sphere; what is left is to divide by the distance.
 template <class T>
 __device__ __forceinline__ void sh_polynomials_vjp(const Directions<T>& d, const Polynomials<T>& o, const T w[kNumSh], T v[3]) {
-    const T x = d.x, y = d.y, z = d.z, xy = o.p[3], yz = o.p[4], xz = o.p[6], c1 = o.p[7];
-    const T w7 = w[7] + w[7], w8 = 3.0f * w[8], w13 = w[13] + w[13], w14 = 3.0f * w[14], xy2 = xy + xy;
+    const T x = d.x, y = d.y, z = d.z, xy2 = o.p[3], yz2 = o.p[4], xz2 = o.p[6], c1 = o.p[7], nyz2 = -1.0f * yz2;
     T gx = fma_(y, w[3], w[2]), gy = fma_(x, w[3], w[0]), gz = fma_(y, w[4], w[1]);
-    gx = fma_(z, w[6], gx); gx = fma_(x, w7, gx); gx = fma_(xy2, w8, gx); gx = fma_(yz, w[9], gx);
-    gx = fma_(o.t, w[12], gx); gx = fma_(xz, w13, gx); gx = fma_(c1, w14, gx);
-    gy = fma_(z, w[4], gy); gy = fma_(c1, w8, gy); gy = fma_(xz, w[9], gy); gy = fma_(o.t, w[10], gy);
-    gy = fma_(-1.0f, fma_(y, w7, fma_(yz, w13, xy2 * w14)), gy);
-    gz = fma_(6.0f * z, w[5], gz); gz = fma_(x, w[6], gz); gz = fma_(xy, w[9], gz);
-    gz = fma_(10.0f, fma_(yz, w[10], xz * w[12]), gz); gz = fma_(fma_(15.0f, z * z, all<T>(-3.0f)), w[11], gz); gz = fma_(c1, w[13], gz);
-    const T ndn = -1.0f * fma_(x, gx, fma_(y, gy, z * gz));
-    v[0] = fma_(x, ndn, gx) * d.inv; v[1] = fma_(y, ndn, gy) * d.inv; v[2] = fma_(z, ndn, gz) * d.inv;
+    gx = fma_(z, w[6], gx); gx = fma_(x, w[7], gx); gx = fma_(xy2, w[8], gx); gx = fma_(yz2, w[9], gx);
+    gx = fma_(o.t, w[12], gx); gx = fma_(xz2, w[13], gx); gx = fma_(c1, w[14], gx);
+    gy = fma_(z, w[4], gy); gy = fma_(o.ny, w[7], gy); gy = fma_(c1, w[8], gy); gy = fma_(xz2, w[9], gy);
+    gy = fma_(o.t, w[10], gy); gy = fma_(nyz2, w[13], gy); gy = fma_(o.x2 * o.ny, w[14], gy);
+    gz = fma_(z, w[5], gz); gz = fma_(x, w[6], gz); gz = fma_(xy2, w[9], gz); gz = fma_(yz2, w[10], gz);
+    gz = fma_(o.t, w[11], gz); gz = fma_(xz2, w[12], gz); gz = fma_(c1, w[13], gz);
+    const T nd = -1.0f * fma_(x, gx, fma_(y, gy, z * gz));
+    v[0] = fma_(x, nd, gx); v[1] = fma_(y, nd, gy); v[2] = fma_(z, nd, gz);
 }
 
 // ---- coefficients ----
@@ -233,7 +246,9 @@ __device__ __forceinline__ constexpr float code_unit(int j) { return 1.0f / (flo
 __device__ __forceinline__ constexpr float code_bias(int j) { return -(8388608.0f + (float)(8 << code_shift(j))); }
 __device__ __forceinline__ float code_bits(const ShRow& r, int j, int ch) {
     const uint32_t w = r.w[2 * ch + (j >> 3)];
-    return __uint_as_float((((j & 7) > 4 ? w >> 16 : w) & (15u << code_shift(j))) | 0x4b000000u);
+    float f;       // (w & mask) | 2^23 in one instruction: left to the compiler it took two
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=f"(f) : "r"((j & 7) > 4 ? w >> 16 : w), "r"(15u << code_shift(j)), "r"(0x4b000000u));
+    return f;
 }
 // (code - 8) / code_unit(j), exact
 __device__ __forceinline__ float code_of(const ShRow& r, int j, int ch) { return code_bits(r, j, ch) + code_bias(j); }
@@ -272,18 +287,19 @@ __device__ __noinline__ void eval_checked(const SsbSplats sp, const float* sh, c
             for (int ch = 0; ch < 3; ++ch) {
                 g[3 + ch] += kShC0 * go[ch];
                 for (int j = 0; j < n_sh; ++j) {
-                    w[j] += sh_constant(j) * W[3 * j + ch] * go[ch];
+                    w[j] += sh_grad_constant(j) * W[3 * j + ch] * go[ch];
                     g[6 + 3 * j + ch] += o.p[j] * sh_constant(j) * go[ch];
                 }
             }
             sh_polynomials_vjp(dir, o, w, vm);
-            for (int k = 0; k < 3; ++k) g[k] += vm[k];
+            for (int k = 0; k < 3; ++k) g[k] += vm[k] * dir.inv;
         }
     }
 }
 
 // ---- one view of 4-bit rows ----
 constexpr int kRowBlock = 128;
+constexpr int kRowBlocksPerSm = 8;
 
 // Components of -centre of view 0 as two floats each, by the block's first three threads; a barrier follows.
 __device__ __forceinline__ void stage_centre(ViewCentre<float>& c, const float* __restrict__ viewmats) {
@@ -294,38 +310,68 @@ __device__ __forceinline__ void stage_centre(ViewCentre<float>& c, const float* 
     }
 }
 
-__global__ void __launch_bounds__(kRowBlock) sh_eval_fwd_row_kernel(SsbSplats sp, const void* __restrict__ rows, int64_t n, const float* __restrict__ viewmats,
-                                                                    int n_sh, float* __restrict__ out) {
+// A splat's inputs; the next tile's are loaded before the current one is worked on.
+struct RowInputs { ShRow r; float mean[3], dc[3]; };
+__device__ __forceinline__ void load_row_inputs(RowInputs& in, const char* rows, const float* means, const float* dc, uint32_t t) {
+    if (rows) in.r = load_sh_row(rows, t);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) in.mean[k] = means[3 * t + k];
+    if (dc)
+#pragma unroll
+        for (int k = 0; k < 3; ++k) in.dc[k] = dc[3 * t + k];
+}
+
+__global__ void __launch_bounds__(kRowBlock, kRowBlocksPerSm) sh_eval_fwd_row_kernel(SsbSplats sp, const void* __restrict__ rows, int64_t n,
+                                                                                     const float* __restrict__ viewmats, int n_sh, float* __restrict__ out) {
     __shared__ ViewCentre<float> centre_s;
-    const int64_t i = (int64_t)blockIdx.x * kRowBlock + threadIdx.x, il = min(i, n - 1);
-    ShRow r = {};
-    if (n_sh > 0) r = load_sh_row(rows, il);
-    const float mean[3] = {sp.means[3 * il], sp.means[3 * il + 1], sp.means[3 * il + 2]};
-    float c[3] = {0.f, 0.f, 0.f};
-    if (sp.features_dc) { c[0] = sp.features_dc[3 * il]; c[1] = sp.features_dc[3 * il + 1]; c[2] = sp.features_dc[3 * il + 2]; }
+    const int64_t first = (int64_t)blockIdx.x * kRowBlock, step = (int64_t)gridDim.x * kRowBlock;
+    // pointers to the tile being loaded, and the splats from its start on
+    const char* rp = n_sh > 0 ? (const char*)rows + kShRowBytes * first : nullptr;
+    const float* mp = sp.means + 3 * first;
+    const float* dp = sp.features_dc ? sp.features_dc + 3 * first : nullptr;
+    float* op = out + 3 * first;
+    int64_t left = n - first;
+    RowInputs in = {};
+    load_row_inputs(in, rp, mp, dp, (uint32_t)min((int64_t)threadIdx.x, left - 1));
     stage_centre(centre_s, viewmats);
     __syncthreads();
-    if (i >= n) return;
-    float d2;
-    const Polynomials<float> o = sh_polynomials(view_directions(centre_s, mean, d2));
+    const ViewCentre<float> centre = centre_s;
+    while (left > 0) {
+        const RowInputs now = in;
+        const bool mine = threadIdx.x < left;
+        left -= step;
+        if (left > 0) {
+            mp += 3 * step;
+            if (rp) rp += kShRowBytes * step;
+            if (dp) dp += 3 * step;
+            load_row_inputs(in, rp, mp, dp, (uint32_t)min((int64_t)threadIdx.x, left - 1));
+        }
+        float d2, c[3];
+        const Polynomials<float> o = sh_polynomials(view_directions(centre, now.mean, d2));
 #pragma unroll
-    for (int ch = 0; ch < 3; ++ch) c[ch] *= kShC0;
+        for (int ch = 0; ch < 3; ++ch) c[ch] = kShC0 * now.dc[ch];
 #pragma unroll
-    for (int b = 0; b < 3; ++b) {
-        float t[3] = {0.f, 0.f, 0.f};
+        for (int b = 0; b < 3; ++b) {
+            float t[3] = {0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < kNumSh; ++j)
-            if (sh_band(j) == b) {
-                const float f = (sh_constant(j) * code_unit(j)) * o.p[j];
+            for (int j = 0; j < kNumSh; ++j)
+                if (sh_band(j) == b) {
+                    const float f = (sh_constant(j) * code_unit(j)) * o.p[j];
 #pragma unroll
-                for (int ch = 0; ch < 3; ++ch) t[ch] = fmaf(f, code_of(r, j, ch), t[ch]);
-            }
-        const float s = active_scale(r, b, n_sh);
+                    for (int ch = 0; ch < 3; ++ch) t[ch] = fmaf(f, code_of(now.r, j, ch), t[ch]);
+                }
+            const float s = active_scale(now.r, b, n_sh);
 #pragma unroll
-        for (int ch = 0; ch < 3; ++ch) c[ch] = fmaf(s, t[ch], c[ch]);
+            for (int ch = 0; ch < 3; ++ch) c[ch] = fmaf(s, t[ch], c[ch]);
+        }
+        if (mine) {
+#pragma unroll
+            for (int ch = 0; ch < 3; ++ch) op[3 * threadIdx.x + ch] = c[ch];
+            if (!(d2 > kSquareMin && d2 < kSquareMax))
+                eval_checked(sp, nullptr, n_sh ? rows : nullptr, (op - out) / 3 + threadIdx.x, n, 1, viewmats, n_sh, out, nullptr, nullptr);
+        }
+        op += 3 * step;
     }
-    out[3 * i] = c[0]; out[3 * i + 1] = c[1]; out[3 * i + 2] = c[2];
-    if (!(d2 > kSquareMin && d2 < kSquareMax)) eval_checked(sp, nullptr, n_sh ? rows : nullptr, i, n, 1, viewmats, n_sh, out, nullptr, nullptr);
 }
 
 __global__ void __launch_bounds__(kRowBlock) sh_eval_bwd_row_kernel(SsbSplats sp, const void* __restrict__ rows, int64_t n, const float* __restrict__ viewmats,
@@ -350,13 +396,13 @@ __global__ void __launch_bounds__(kRowBlock) sh_eval_bwd_row_kernel(SsbSplats sp
         t = fmaf(code_of(r, j, 1), g[1], t);
         t = fmaf(code_of(r, j, 2), g[2], t);
         const bool active = n_sh > (sh_band(j) + 1) * (sh_band(j) + 1) - 1;
-        w[j] = active ? ((sh_constant(j) * code_unit(j)) * sh_row_scale(r, sh_band(j))) * t : 0.0f;
+        w[j] = active ? ((sh_grad_constant(j) * code_unit(j)) * sh_row_scale(r, sh_band(j))) * t : 0.0f;
 #pragma unroll
         for (int ch = 0; ch < 3; ++ch) sh_s[threadIdx.x * kShPerSplat + 3 * j + ch] = active ? sh_constant(j) * o.p[j] * g[ch] : 0.0f;
     }
     sh_polynomials_vjp(d, o, w, vm);
 #pragma unroll
-    for (int k = 0; k < 3; ++k) { mean_s[3 * threadIdx.x + k] = vm[k]; dc_s[3 * threadIdx.x + k] = kShC0 * g[k]; }
+    for (int k = 0; k < 3; ++k) { mean_s[3 * threadIdx.x + k] = vm[k] * d.inv; dc_s[3 * threadIdx.x + k] = kShC0 * g[k]; }
     if (!(d2 > kSquareMin && d2 < kSquareMax)) {
         float e[6 + kShPerSplat];
         eval_checked(sp, nullptr, n_sh ? rows : nullptr, il, n, 1, viewmats, n_sh, nullptr, v_out, e);
@@ -394,15 +440,46 @@ __device__ __forceinline__ void stage_tile(float* sh_s, unsigned char* raw_s, co
     __syncthreads();
 }
 
-// k_j W[j][ch] of both splats, zero above the active degree.
+// A tile's inputs travel to shared memory while the tile before is worked on: each thread copies and reads its own two splats', so
+// no barrier is needed.
+struct TileInputs { uint4 row[4][kProjBlock]; Pair mean[3][kProjBlock], dc[3][kProjBlock]; };
+__device__ __forceinline__ void fetch_pairs(const Pair* dst, const float* __restrict__ p, int64_t l0, int64_t l1) {
+    const uint32_t s = (uint32_t)__cvta_generic_to_shared(dst);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s + 8 * kProjBlock * k), "l"(p + 3 * l0 + k) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s + 8 * kProjBlock * k + 4), "l"(p + 3 * l1 + k) : "memory");
+    }
+}
 template <bool ROWS>
-__device__ __forceinline__ void read_coefficients(Pair W[kShPerSplat], const float* sh_s, const void* rows, int64_t i0, int64_t i1, int n_sh) {
+__device__ __forceinline__ void fetch_inputs(TileInputs& in, const SsbSplats& sp, bool want_dc, const void* __restrict__ rows, int n_sh, int64_t first, int64_t n) {
+    if (first < n) {
+        const int64_t l0 = min(first + threadIdx.x, n - 1), l1 = min(first + threadIdx.x + kProjBlock, n - 1);
+        if (ROWS && n_sh > 0) {
+            const uint32_t s = (uint32_t)__cvta_generic_to_shared(&in.row[0][threadIdx.x]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s + 16 * kProjBlock * k),
+                             "l"((const char*)rows + kShRowBytes * (k < 2 ? l0 : l1) + 16 * (k & 1)) : "memory");
+        }
+        fetch_pairs(&in.mean[0][threadIdx.x], sp.means, l0, l1);
+        if (want_dc) fetch_pairs(&in.dc[0][threadIdx.x], sp.features_dc, l0, l1);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ ShRow input_row(const TileInputs& in, int which) {
+    const uint4 a = in.row[2 * which][threadIdx.x], b = in.row[2 * which + 1][threadIdx.x];
+    return ShRow{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+}
+
+// W[j][ch] of both splats times sh_constant(j) or, for the backward pass, sh_grad_constant(j); zero above the active degree.
+template <bool ROWS, bool GRAD>
+__device__ __forceinline__ void read_coefficients(Pair W[kShPerSplat], const float* sh_s, const TileInputs& in, int n_sh) {
     if (ROWS) {
-        ShRow a = {}, b = {};
-        if (n_sh > 0) { a = load_sh_row(rows, i0); b = load_sh_row(rows, i1); }
+        const ShRow a = input_row(in, 0), b = input_row(in, 1);
 #pragma unroll
         for (int j = 0; j < kNumSh; ++j) {
-            const Pair f = (sh_constant(j) * code_unit(j)) * make_float2(active_scale(a, sh_band(j), n_sh), active_scale(b, sh_band(j), n_sh));
+            const Pair f = ((GRAD ? sh_grad_constant(j) : sh_constant(j)) * code_unit(j)) * make_float2(active_scale(a, sh_band(j), n_sh), active_scale(b, sh_band(j), n_sh));
 #pragma unroll
             for (int ch = 0; ch < 3; ++ch) W[3 * j + ch] = f * code_of(a, b, j, ch);
         }
@@ -412,15 +489,26 @@ __device__ __forceinline__ void read_coefficients(Pair W[kShPerSplat], const flo
 #pragma unroll
             for (int ch = 0; ch < 3; ++ch) {
                 const int k = 3 * j + ch;
-                W[k] = j < n_sh ? sh_constant(j) * make_float2(sh_s[threadIdx.x * kShPerSplat + k], sh_s[(threadIdx.x + kProjBlock) * kShPerSplat + k])
+                W[k] = j < n_sh ? (GRAD ? sh_grad_constant(j) : sh_constant(j)) * make_float2(sh_s[threadIdx.x * kShPerSplat + k], sh_s[(threadIdx.x + kProjBlock) * kShPerSplat + k])
                                 : all<Pair>(0.0f);
             }
     }
 }
 
-__device__ __forceinline__ void load_pairs(const float* __restrict__ p, int64_t i0, int64_t i1, Pair v[3]) {
+// The sum over j as a polynomial in z whose coefficients belong to the azimuthal functions 1, x, y, x^2 - y^2, 2xy, x^3 - 3xy^2 and
+// 3x^2 y - y^3: fifteen multiply-adds like the sum itself, but the fifteen p_j need not be formed, only the azimuthal functions.
+// W comes in as sh_constant(j) W_j and leaves as: [0] z^3 [1] z^2 [2] z [3] 1 (with dc) | [4] x z^2 [5] x z [6] x | [7] y z^2 [8] y z
+// [9] y | [10] (x^2 - y^2) z [11] x^2 - y^2 | [12] 2xy z [13] 2xy | [14] x^3 - 3xy^2 [15] 3x^2 y - y^3, of channel ch at 3 * k + ch.
+__device__ __forceinline__ void to_azimuthal(Pair A[16 * 3], const Pair W[kShPerSplat], const Pair dc[3]) {
 #pragma unroll
-    for (int k = 0; k < 3; ++k) v[k] = make_float2(p[3 * i0 + k], p[3 * i1 + k]);
+    for (int ch = 0; ch < 3; ++ch) {
+        A[0 + ch] = W[33 + ch]; A[3 + ch] = W[15 + ch]; A[6 + ch] = fma_(-0.6f, W[33 + ch], W[3 + ch]); A[9 + ch] = fma_(-1.0f / 3.0f, W[15 + ch], dc[ch]);
+        A[12 + ch] = W[36 + ch]; A[15 + ch] = W[18 + ch] + W[18 + ch]; A[18 + ch] = fma_(-0.2f, W[36 + ch], W[6 + ch]);
+        A[21 + ch] = W[30 + ch]; A[24 + ch] = W[12 + ch] + W[12 + ch]; A[27 + ch] = fma_(-0.2f, W[30 + ch], W[0 + ch]);
+        A[30 + ch] = W[39 + ch]; A[33 + ch] = W[21 + ch];
+        A[36 + ch] = W[27 + ch]; A[39 + ch] = W[9 + ch];
+        A[42 + ch] = W[42 + ch]; A[45 + ch] = W[24 + ch];
+    }
 }
 
 constexpr int kFwdBlocksPerSm = 3, kBwdBlocksPerSm = 2;       // what their registers allow; the grids are this many blocks
@@ -431,23 +519,27 @@ __global__ void __launch_bounds__(kProjBlock, kFwdBlocksPerSm) sh_eval_fwd_views
                                                                                         float* __restrict__ out) {
     extern __shared__ __align__(16) unsigned char dyn_s[];
     __shared__ ViewCentre<Pair> centres_s[kCentreChunk];
+    __shared__ TileInputs in;
     float* sh_s = (float*)dyn_s;
+    const bool with_dc = sp.features_dc != nullptr;
+    const int64_t stride = (int64_t)gridDim.x * kEvalTile;
+    fetch_inputs<ROWS>(in, sp, with_dc, shq.packed, n_sh, (int64_t)blockIdx.x * kEvalTile, n);
     stage_centres(centres_s, viewmats, 0, views);
     __syncthreads();
-    for (int64_t first = (int64_t)blockIdx.x * kEvalTile; first < n; first += (int64_t)gridDim.x * kEvalTile) {
-        const int64_t i0 = first + threadIdx.x, i1 = i0 + kProjBlock, l0 = min(i0, n - 1), l1 = min(i1, n - 1);
+    for (int64_t first = (int64_t)blockIdx.x * kEvalTile; first < n; first += stride) {
+        const int64_t i0 = first + threadIdx.x, i1 = i0 + kProjBlock;
         if (!ROWS) {
             __syncthreads();
             stage_tile(sh_s, dyn_s + kEvalShBytes, sp, shq, first, n);
         }
-        Pair mean[3], dc[3] = {all<Pair>(0.f), all<Pair>(0.f), all<Pair>(0.f)}, W[kShPerSplat];
-        load_pairs(sp.means, l0, l1, mean);
-        if (sp.features_dc) {
-            load_pairs(sp.features_dc, l0, l1, dc);
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        Pair mean[3], dc[3], W[kShPerSplat];
 #pragma unroll
-            for (int ch = 0; ch < 3; ++ch) dc[ch] = kShC0 * dc[ch];
-        }
-        read_coefficients<ROWS>(W, sh_s, shq.packed, l0, l1, n_sh);
+        for (int k = 0; k < 3; ++k) { mean[k] = in.mean[k][threadIdx.x]; dc[k] = with_dc ? kShC0 * in.dc[k][threadIdx.x] : all<Pair>(0.f); }
+        read_coefficients<ROWS, false>(W, sh_s, in, n_sh);
+        Pair A[16 * 3];
+        to_azimuthal(A, W, dc);
+        fetch_inputs<ROWS>(in, sp, with_dc, shq.packed, n_sh, first + stride, n);
         float least = kSquareMax, most = kSquareMin;
         for (int v0 = 0; v0 < views; v0 += kCentreChunk) {
             if (views > kCentreChunk) {
@@ -458,13 +550,20 @@ __global__ void __launch_bounds__(kProjBlock, kFwdBlocksPerSm) sh_eval_fwd_views
             const int v1 = min(views - v0, kCentreChunk);
             float* o0 = out + 3 * ((int64_t)v0 * n + i0);
             for (int v = 0; v < v1; ++v, o0 += 3 * n) {
-                Pair d2, c[3] = {dc[0], dc[1], dc[2]};
-                const Polynomials<Pair> o = sh_polynomials(view_directions(centres_s[v], mean, d2));
+                Pair d2, c[3];
+                const Directions<Pair> d = view_directions(centres_s[v], mean, d2);
                 least = fminf(least, fminf(d2.x, d2.y)); most = fmaxf(most, fmaxf(d2.x, d2.y));
+                const Pair ny = -1.0f * d.y, c1 = fma_(d.x, d.x, ny * d.y), s1 = (d.x + d.x) * d.y;
+                const Pair c3 = fma_(d.x, c1, ny * s1), s3 = fma_(d.x, s1, d.y * c1);
 #pragma unroll
-                for (int j = 0; j < kNumSh; ++j)
-#pragma unroll
-                    for (int ch = 0; ch < 3; ++ch) c[ch] = fma_(o.p[j], W[3 * j + ch], c[ch]);
+                for (int ch = 0; ch < 3; ++ch) {
+                    Pair t = fma_(d.z, fma_(d.z, fma_(d.z, A[ch], A[3 + ch]), A[6 + ch]), A[9 + ch]);
+                    t = fma_(d.x, fma_(d.z, fma_(d.z, A[12 + ch], A[15 + ch]), A[18 + ch]), t);
+                    t = fma_(d.y, fma_(d.z, fma_(d.z, A[21 + ch], A[24 + ch]), A[27 + ch]), t);
+                    t = fma_(c1, fma_(d.z, A[30 + ch], A[33 + ch]), t);
+                    t = fma_(s1, fma_(d.z, A[36 + ch], A[39 + ch]), t);
+                    c[ch] = fma_(s3, A[45 + ch], fma_(c3, A[42 + ch], t));
+                }
 #pragma unroll
                 for (int ch = 0; ch < 3; ++ch) {
                     if (i0 < n) o0[ch] = c[ch].x;
@@ -483,17 +582,26 @@ __global__ void __launch_bounds__(kProjBlock, kFwdBlocksPerSm) sh_eval_fwd_views
 // The gradients of the next views travel to shared memory while a view is worked on: each thread copies and reads its own six
 // numbers, so no barrier is needed.
 constexpr int kGradAhead = 3;
-struct GradRing { float g[kGradAhead + 1][3][kEvalTile]; };
-__device__ __forceinline__ void fetch_grads(GradRing& ring, const float* __restrict__ v_out, int64_t n, int v, int views, int64_t l0, int64_t l1) {
-    if (v < views) {
-        const float* p = v_out + 3 * (int64_t)v * n;
-        float* q = &ring.g[v & kGradAhead][0][threadIdx.x];
-        const uint32_t s = (uint32_t)__cvta_generic_to_shared(q);
+struct GradRing { Pair g[kGradAhead + 1][3][kProjBlock]; };
+// What the ring fetches next: view after view of a tile, then on into the block's next tile.
+struct GradCursor { const float* p0; const float* p1; int64_t first; int view; };
+__device__ __forceinline__ void cursor_tile(GradCursor& c, const float* v_out, int64_t n, int64_t first) {
+    c.first = first;
+    c.view = 0;
+    c.p0 = v_out + 3 * min(first + threadIdx.x, n - 1);
+    c.p1 = v_out + 3 * min(first + threadIdx.x + kProjBlock, n - 1);
+}
+__device__ __forceinline__ void fetch_grads(GradRing& ring, int slot, GradCursor& c, const float* v_out, int64_t n, int views, int64_t stride) {
+    if (c.first < n) {
+        const uint32_t s = (uint32_t)__cvta_generic_to_shared(&ring.g[slot][0][threadIdx.x]);
 #pragma unroll
         for (int k = 0; k < 3; ++k) {
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s + 4 * kEvalTile * k), "l"(p + 3 * l0 + k) : "memory");
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s + 4 * kEvalTile * k + 4 * kProjBlock), "l"(p + 3 * l1 + k) : "memory");
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s + 8 * kProjBlock * k), "l"(c.p0 + k) : "memory");
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(s + 8 * kProjBlock * k + 4), "l"(c.p1 + k) : "memory");
         }
+        c.p0 += 3 * n;
+        c.p1 += 3 * n;
+        if (++c.view == views) cursor_tile(c, v_out, n, c.first + stride);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
 }
@@ -506,18 +614,28 @@ __global__ void __launch_bounds__(kProjBlock, kBwdBlocksPerSm) sh_eval_bwd_views
     __shared__ __align__(16) float mean_s[kEvalTile * 3];
     __shared__ __align__(16) float dc_s[kEvalTile * 3];
     __shared__ GradRing ring;
+    __shared__ TileInputs in;
     __shared__ ViewCentre<Pair> centres_s[kCentreChunk];
     float* sh_s = (float*)dyn_s;                 // values on the way in, their gradients on the way out
+    const int64_t stride = (int64_t)gridDim.x * kEvalTile;
+    GradCursor ahead;
+    int slot = 0;
+    cursor_tile(ahead, v_out, n, (int64_t)blockIdx.x * kEvalTile);
+    fetch_inputs<ROWS>(in, sp, false, shq.packed, n_sh, (int64_t)blockIdx.x * kEvalTile, n);
+    for (int k = 0; k < kGradAhead && views > 0; ++k) fetch_grads(ring, k, ahead, v_out, n, views, stride);
     stage_centres(centres_s, viewmats, 0, views);
-    for (int64_t first = (int64_t)blockIdx.x * kEvalTile; first < n; first += (int64_t)gridDim.x * kEvalTile) {
+    for (int64_t first = (int64_t)blockIdx.x * kEvalTile; first < n; first += stride) {
         const int64_t i0 = first + threadIdx.x, i1 = i0 + kProjBlock, l0 = min(i0, n - 1), l1 = min(i1, n - 1);
         __syncthreads();
         if (!ROWS) stage_tile(sh_s, dyn_s + kEvalShBytes, sp, shq, first, n);
-#pragma unroll
-        for (int v = 0; v < kGradAhead; ++v) fetch_grads(ring, v_out, n, v, views, l0, l1);
+        // at least `views` groups were begun after the tile's inputs, the last kGradAhead of which may be under way
+        if (views >= kGradAhead) asm volatile("cp.async.wait_group %0;" ::"n"(kGradAhead) : "memory");
+        else asm volatile("cp.async.wait_group 0;" ::: "memory");
         Pair mean[3], g_mean[3], g_dc[3], g_sh[kShPerSplat], W[kShPerSplat];
-        load_pairs(sp.means, l0, l1, mean);
-        read_coefficients<ROWS>(W, sh_s, shq.packed, l0, l1, n_sh);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) mean[k] = in.mean[k][threadIdx.x];
+        read_coefficients<ROWS, true>(W, sh_s, in, n_sh);
+        fetch_inputs<ROWS>(in, sp, false, shq.packed, n_sh, first + stride, n);
 #pragma unroll
         for (int k = 0; k < 3; ++k) g_mean[k] = g_dc[k] = all<Pair>(0.f);
 #pragma unroll
@@ -532,11 +650,11 @@ __global__ void __launch_bounds__(kProjBlock, kBwdBlocksPerSm) sh_eval_bwd_views
             const int v1 = min(views - v0, kCentreChunk);
             for (int v = 0; v < v1; ++v) {
                 Pair d2, g[3], w[kNumSh], vm[3];
-                fetch_grads(ring, v_out, n, v0 + v + kGradAhead, views, l0, l1);
+                fetch_grads(ring, (slot + kGradAhead) & kGradAhead, ahead, v_out, n, views, stride);
                 asm volatile("cp.async.wait_group %0;" ::"n"(kGradAhead) : "memory");
 #pragma unroll
-                for (int k = 0; k < 3; ++k)
-                    g[k] = make_float2(ring.g[(v0 + v) & kGradAhead][k][threadIdx.x], ring.g[(v0 + v) & kGradAhead][k][threadIdx.x + kProjBlock]);
+                for (int k = 0; k < 3; ++k) g[k] = ring.g[slot][k][threadIdx.x];
+                slot = (slot + 1) & kGradAhead;
                 const Directions<Pair> d = view_directions(centres_s[v], mean, d2);
                 const Polynomials<Pair> o = sh_polynomials(d);
                 least = fminf(least, fminf(d2.x, d2.y)); most = fmaxf(most, fmaxf(d2.x, d2.y));
@@ -550,7 +668,7 @@ __global__ void __launch_bounds__(kProjBlock, kBwdBlocksPerSm) sh_eval_bwd_views
                 }
                 sh_polynomials_vjp(d, o, w, vm);
 #pragma unroll
-                for (int k = 0; k < 3; ++k) { g_dc[k] = fma_(kShC0, g[k], g_dc[k]); g_mean[k] = g_mean[k] + vm[k]; }
+                for (int k = 0; k < 3; ++k) { g_dc[k] = g_dc[k] + g[k]; g_mean[k] = fma_(vm[k], d.inv, g_mean[k]); }
             }
         }
         float e0[6 + kShPerSplat], e1[6 + kShPerSplat];
@@ -567,7 +685,7 @@ __global__ void __launch_bounds__(kProjBlock, kBwdBlocksPerSm) sh_eval_bwd_views
 #pragma unroll
         for (int k = 0; k < 3; ++k) {
             mean_s[3 * t0 + k] = g_mean[k].x; mean_s[3 * t1 + k] = g_mean[k].y;
-            dc_s[3 * t0 + k] = g_dc[k].x; dc_s[3 * t1 + k] = g_dc[k].y;
+            dc_s[3 * t0 + k] = kShC0 * g_dc[k].x; dc_s[3 * t1 + k] = kShC0 * g_dc[k].y;
         }
 #pragma unroll
         for (int j = 0; j < kNumSh; ++j)
@@ -621,7 +739,7 @@ int ssb_sh_eval_fwd(const SsbSplats* splats, const SsbShQuant* shq, int64_t n, c
     cudaStream_t st = (cudaStream_t)stream;
     const bool rows = q.bits == 4 || n_sh == 0;
     if (rows && cams->count == 1) {
-        sh_eval_fwd_row_kernel<<<(unsigned)ceil_div(n, kRowBlock), kRowBlock, 0, st>>>(*splats, q.packed, n, cams->d_viewmats, n_sh, d_values);
+        sh_eval_fwd_row_kernel<<<(unsigned)std::min<int64_t>(ceil_div(n, kRowBlock), 148 * kRowBlocksPerSm), kRowBlock, 0, st>>>(*splats, q.packed, n, cams->d_viewmats, n_sh, d_values);
     } else {
         const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(n, kEvalTile), 148 * kFwdBlocksPerSm);
         constexpr int smem = kEvalShBytes + kShRawBytes;
