@@ -138,7 +138,7 @@ struct OpacityArgs {
 // 1 - e^-d for d > 0 to within 2^-22.  Below 1.375 as d P(d), P the polynomial of degree seven that fits (1 - e^-d) / d there
 // (Chebyshev nodes; 2^-29.8 off, 2.7 half-ulps as evaluated); above it the hardware exponential, whose 2 ulp and the
 // argument's rounding weigh e^-d / (1 - e^-d) <= 0.34 of themselves.  Other d are not used (the opacity is then limited).  expm1f
-// measured 68 against 55 us for 10M opacities, forward and backward.
+// instead made the two calls take 68 instead of 55 us for 10M opacities.
 __device__ __forceinline__ float one_minus_exp_neg(float d) {
     float p = -1.36514881887706e-05f;
     p = fmaf(p, d, 0.0001761570747476071f);
@@ -157,7 +157,11 @@ template <bool BWD>
 __device__ __forceinline__ float drop_opacity(float x, float v, bool dropped, const OpacityArgs& o) {
     const float w = one_minus_exp_neg((o.x0_hi - x) + o.x0_lo);
     if (BWD) return (dropped || x > o.x_cap) ? 0.0f : __fdividef(v, w);
-    return dropped ? kDroppedLogit : (x > o.x_cap ? o.capped : (x + o.a) - logf(w));
+    // the hardware logarithm: off by 2^-22 where w is above 1/2 and by 2^-22 of itself below, against w's own 2^-22; logf made
+    // the forward call take 29 instead of 21 us for 10M opacities
+    float l;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(l) : "f"(w));
+    return dropped ? kDroppedLogit : (x > o.x_cap ? o.capped : fmaf(-0.6931471805599453f, l, x + o.a));
 }
 
 constexpr int kOpacityChunks = 2;

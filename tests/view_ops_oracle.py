@@ -54,9 +54,10 @@ def dropout_opacities(x, first, rate, seed, offset):
         y = np.where(capped, np.log(CAP / (1.0 - CAP)), x + a - lw)
         slope = np.where(capped, 0.0, (e + r) / e)
         slope = np.where(np.isposinf(e), 1.0, slope)
-        # ln w: w = 1 - e^-d with d off by 2 U relative and expm1f by one ulp (2 U), together 4 U relative in w; logf one ulp
-        # (2 U); then the rounding of a, of x + a and of the difference
-        bound = np.where(capped, U * np.abs(y), U * (4.0 + 2.0 * np.abs(lw) + a + np.abs(x + a) + np.abs(y)))
+        # ln w: w = 1 - e^-d with d off by 2 U relative, which w / (e^d - 1) d <= 1 hands on, and 1 - e^-d by another 2 U relative,
+        # together 4 U relative in w; a base-2 logarithm off by 2^-22 = 4 U absolute above w = 1/2 and relative below, times ln 2
+        # (itself half a U off); then the rounding of a, of x + a and of the final multiply-add
+        bound = np.where(capped, U * np.abs(y), U * (4.0 + np.maximum(4.0 * np.log(2.0), 4.0 * np.abs(lw)) + 0.5 * np.abs(lw) + a + np.abs(x + a) + np.abs(y)))
     y = np.where(d, DROPPED, y)
     return y, np.where(d, 0.0, slope), np.where(d, 0.0, bound)
 
