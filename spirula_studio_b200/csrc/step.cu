@@ -488,6 +488,7 @@ static int project_bwd_optimize_impl(const SsbSplats* params, const SsbShQuant* 
     SSB_REQUIRE(params && cams && d_aabb && d_v_screen && cfg && d_workspace, "ssb_project_bwd_optimize: NULL argument");
     SSB_REQUIRE(nq ? (sh_state || (m1 && m2 && m1->features_sh && m2->features_sh)) : (m1 && m2),
                 "ssb_project_bwd_optimize: moments missing (with 16-bit moments m1 / m2 carry features_sh, unless the SH state is quantised)");
+    SSB_REQUIRE(!nq || sh_state || params->features_sh, "ssb_project_bwd_optimize: no SH values to update (params->features_sh or sh_state)");
     SSB_REQUIRE(n >= 0 && cams->count >= 0, "ssb_project_bwd_optimize: bad sizes");
     SSB_REQUIRE(workspace_bytes >= ssb_project_bwd_optimize_workspace_bytes(n), "ssb_project_bwd_optimize: workspace too small");
     SSB_REQUIRE(((uintptr_t)d_workspace & 255) == 0, "ssb_project_bwd_optimize: the workspace must be 256-byte aligned");
@@ -526,6 +527,7 @@ static int step_backward_optimize_impl(SsbStep* s, const SsbSplats* params, cons
     SSB_REQUIRE(s && params && d_viewmats && d_intrins && cfg, "ssb_step_backward_optimize: NULL argument");
     SSB_REQUIRE(nq ? (sh_state || (m1 && m2 && m1->features_sh && m2->features_sh)) : (m1 && m2),
                 "ssb_step_backward_optimize: moments missing (with 16-bit moments m1 / m2 carry features_sh, unless the SH state is quantised)");
+    SSB_REQUIRE(!nq || sh_state || params->features_sh, "ssb_step_backward_optimize: no SH values to update (params->features_sh or sh_state)");
     SSB_REQUIRE(s->def_max_views > 0, "ssb_step_backward_optimize: the step does not keep its views (ssb_step_set_fused_backward)");
     SSB_REQUIRE(n_views == s->def_count && n_views <= s->def_max_views, "ssb_step_backward_optimize: %d views given, %d kept (room for %d)", n_views,
                 s->def_count, s->def_max_views);

@@ -163,3 +163,15 @@ def test_sh_eval_refusals():
     assert fwd(n=0) == L.SSB_OK and bwd(n=0) == L.SSB_OK
     c = L.SsbCameras()
     assert fwd(c=c) == L.SSB_OK                                                        # no views
+
+
+def test_fused_backward_without_sh_values_to_update_is_refused():
+    """Views may read rows while the fp32 values are absent, but then the 16-bit-moment step has nothing to update."""
+    lib = L.load()
+    sp, cams, m, cfg = L.SsbSplats(), L.SsbCameras(), L.SsbSplats(), L.SsbAdamConfig(0, 0, 0, 0, 0, 1e-3, 0, 1, 1, 0)
+    m.features_sh = 64
+    q16, rows = L.SsbMomentsQ16(), L.SsbShQuant(64, None, 4, 0, 0)
+    ws = C.c_void_p(256)
+    assert lib.ssb_project_bwd_optimize_q16(C.byref(sp), C.byref(rows), 1000, C.byref(cams), ONE, ONE, C.byref(q16), C.byref(m), C.byref(m), None,
+                                            C.byref(cfg), None, ws, 1 << 30, None) == L.SSB_ERR_INVALID_ARGUMENT
+    assert b"SH values" in lib.ssb_last_error_string()
