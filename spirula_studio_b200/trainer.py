@@ -212,7 +212,7 @@ class Trainer:
             raise ValueError("view_sh_bits=4 needs fp32 SH values (sh_value_bits = 32)")
         self.view_sh_bits = view_sh_bits
         self.dropout = None
-        self._view_opacities = self._view_sh = self._sh_rows = None
+        self._view_opacities = self._view_sh = self._sh_rows = self._render_rows = None
         self._dropped = None                 # this iteration's (splat, SH) descriptions between its views and its optimiser step
         self._v_struct, self._v_shq = self._p_struct, self.shq
         self._views_open = False
@@ -387,7 +387,7 @@ class Trainer:
         own = sum(t.numel() * t.element_size() for t in (self.params_flat, self.grads_flat, self.m1_flat, self.m2_flat))
         if self.quant:
             own += sum(t.numel() * t.element_size() for t in (self.sh_packed, self.sh_bounds, self.sh_optim_packed, self.sh_optim_bounds))
-        own += sum(t.numel() * t.element_size() for t in (self._view_opacities, self._view_sh, self._sh_rows) if t is not None)
+        own += sum(t.numel() * t.element_size() for t in (self._view_opacities, self._view_sh, self._sh_rows, self._render_rows) if t is not None)
         return own + sum(int(self.lib.ssb_step_device_bytes(h)) for h in self.handles)
 
     # -- pieces ------------------------------------------------------------
@@ -419,11 +419,12 @@ class Trainer:
             raise ValueError(f"sh_group must be at least 1, not {self.dropout.sh_group}")
         self.dropout.splat_rate, self.dropout.sh_rate = float(splat_rate), float(sh_rate)
 
-    def _encode_rows(self, values, stream=None):
-        if self._sh_rows is None:
-            self._sh_rows = torch.empty(self.n * L.SH_ROW_BYTES, dtype=torch.uint8, device=self.device)
-        L.check(self.lib.ssb_quant_encode(L.ptr(values), self.n * 45, 4, L.ptr(self._sh_rows), None, stream))
-        return L.shq_struct(self._sh_rows, None, 4, 0)
+    def _encode_rows(self, values, rows, stream=None):
+        """values in 4-bit rows: into `rows`, or a new buffer; returns (rows, their SsbShQuant)."""
+        if rows is None:
+            rows = torch.empty(self.n * L.SH_ROW_BYTES, dtype=torch.uint8, device=self.device)
+        L.check(self.lib.ssb_quant_encode(L.ptr(values), self.n * 45, 4, L.ptr(rows), None, stream))
+        return rows, L.shq_struct(rows, None, 4, 0)
 
     def _begin_views(self, stream=None):
         """Before an iteration's first view: makes the arrays its views read."""
@@ -445,7 +446,7 @@ class Trainer:
             L.check(self.lib.ssb_dropout(L.ptr(self.params["features_sh"]), 0, self.n * 45, d.sh_group, C.byref(sh), L.ptr(self._view_sh), stream))
             views["features_sh"] = self._view_sh
         if self.view_sh_bits == 4:
-            shq = self._encode_rows(views["features_sh"], stream)
+            self._sh_rows, shq = self._encode_rows(views["features_sh"], self._sh_rows, stream)
         if splat is not None or sh is not None:
             self._dropped = (splat, sh, d.sh_group)
             self._v_struct = L.splats_struct(views)
@@ -483,7 +484,9 @@ class Trainer:
         T = torch.empty(height, width, device=self.device)
         dep = torch.empty(height, width, device=self.device) if depth else None
         stream = C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
-        shq = self._encode_rows(self.params["features_sh"], stream) if sh_bits == 4 else self.shq
+        shq = self.shq
+        if sh_bits == 4:        # a buffer of its own: an iteration's views may be under way on theirs
+            self._render_rows, shq = self._encode_rows(self.params["features_sh"], self._render_rows, stream)
         L.check(self.lib.ssb_step_render(self.handles[kind], C.byref(self._p_struct), C.byref(shq) if shq else None, L.ptr(d_vm), L.ptr(d_K),
                                          L.ptr(rgb), L.ptr(dep) if depth else None, L.ptr(T), stream))
         return (rgb, T, dep) if depth else (rgb, T)

@@ -226,6 +226,98 @@ def test_rows_with_dropout_and_with_the_fused_backward(lib):
         t.close()
 
 
+def test_rendering_between_the_views_of_an_iteration_changes_nothing(lib):
+    cfg, sp, vm, K, gt = scene(n=2500)
+    opts = DropoutOptions(splat_rate=0.2, sh_rate=0.4, seed=9)
+    grads = []
+    for render in (False, True):
+        tr = Trainer(cfg, sp, device=DEV, view_sh_bits=4, dropout=opts)
+        tr.views_fwd_bwd(dev(vm[:1]), dev(K[:1]), dev(gt[:1]), 1)
+        if render:
+            tr.render(vm[0], K[0])
+        tr.views_fwd_bwd(dev(vm[1:]), dev(K[1:]), dev(gt[1:]), 2, accumulate=True)
+        tr.optimizer_step(3)              # without allreduce_grads: the step itself ends the views
+        torch.cuda.synchronize()
+        grads.append({k: v.clone() for k, v in tr.grads.items()})
+        tr.close()
+    for k in grads[0]:
+        assert close(grads[1][k], grads[0][k]), k
+    drop = O.dropped(0, 2500 * 45, 3, 0.4, 19, 0)
+    assert not grads[0]["features_sh"][dev(drop)].any()
+    # gradient accumulation into a caller's own zeroed buffer, the first call already accumulating
+    tr = Trainer(cfg, sp, device=DEV, view_sh_bits=4, dropout=opts)
+    tr.views_fwd_bwd(dev(vm), dev(K), dev(gt), 3, accumulate=True)
+    tr.allreduce_grads()
+    torch.cuda.synchronize()
+    for k in grads[0]:
+        assert close(tr.grads[k], grads[0][k]), k
+    tr.close()
+
+
+def test_dropout_with_a_densifier_and_a_checkpoint(lib, tmp_path):
+    """The stored parameters, not the dropped ones, are densified, saved and resumed; a resumed trainer draws the same masks."""
+    from spirula_studio_b200 import checkpoint as ck
+    cfg, sp, vm, K, gt = scene(n=2000)
+    opts = DropoutOptions(splat_rate=0.3, sh_rate=0.3, seed=4)
+    h = pinned(vm, K, gt)
+    a = Trainer(cfg, sp, device=DEV, view_sh_bits=4, dropout=opts)
+    for _ in range(2):
+        a.train_step(*h, 3)
+    ck.save_checkpoint(a, str(tmp_path))
+    b = Trainer(cfg, sp, device=DEV, view_sh_bits=4, dropout=opts)
+    ck.load_checkpoint(b, str(tmp_path))
+    assert b.iteration == 2 and torch.equal(a.params["opacities"], b.params["opacities"])
+    la, lb = a.train_step(*h, 3), b.train_step(*h, 3)
+    assert abs(la[2] - lb[2]) <= 1e-5 * abs(la[2])
+    drop = O.dropped(0, 2000, 1, 0.3, 8, 2)
+    for t in (a, b):
+        assert not t.grads["means"].view(2000, 3)[dev(drop)].any()
+    for k in a.grads:
+        assert close(a.grads[k], b.grads[k]), k
+    a.close(); b.close()
+
+
+def test_first_calls_inside_a_capture():
+    """A fresh process whose first call of every entry point happens while a stream is being captured."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import ctypes as C, torch
+from spirula_studio_b200 import lib as L
+lib = L.load()
+n, V = 500, 3
+x = torch.randn(n * 45, device="cuda"); y = torch.zeros_like(x); rows = torch.zeros(n, 32, dtype=torch.uint8, device="cuda")
+m = torch.randn(n, 3, device="cuda"); vm = torch.eye(4, device="cuda").reshape(1, 16).repeat(V, 1).contiguous()
+out = torch.zeros(V, n, 3, device="cuda"); g = torch.zeros(n, 45, device="cuda"); gm = torch.zeros(n, 3, device="cuda")
+d = L.dropout_struct(0.3, 1, 2)
+sp = L.splats_struct(dict(means=m)); spf = L.splats_struct(dict(means=m, features_sh=y)); gr = L.splats_struct(dict(means=gm, features_sh=g))
+q = L.shq_struct(rows, None, 4, 0)
+cams = L.cameras_struct(vm, vm, 1, 1); one = L.cameras_struct(vm, vm, 1, 1, count=1)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    st = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    L.check(lib.ssb_dropout(L.ptr(x), 0, n * 45, 3, C.byref(d), L.ptr(y), st))
+    L.check(lib.ssb_dropout(L.ptr(y), 0, n * 45, 1, C.byref(d), L.ptr(y), st))
+    L.check(lib.ssb_dropout_opacities(L.ptr(x), 0, n, C.byref(d), L.ptr(gm), st))
+    L.check(lib.ssb_dropout_opacities_bwd(L.ptr(x), L.ptr(x), 0, n, C.byref(d), L.ptr(gm), st))
+    L.check(lib.ssb_quant_encode(L.ptr(y), n * 45, 4, L.ptr(rows), None, st))
+    L.check(lib.ssb_quant_decode(L.ptr(rows), None, n * 45, 4, L.ptr(g), st))
+    for s, shq in ((sp, C.byref(q)), (spf, None)):
+        for c in (one, cams):
+            L.check(lib.ssb_sh_eval_fwd(C.byref(s), shq, n, C.byref(c), L.ptr(out), st))
+            L.check(lib.ssb_sh_eval_bwd(C.byref(s), shq, n, C.byref(c), L.ptr(out), C.byref(gr), 0, st))
+graph.replay()
+torch.cuda.synchronize()
+assert torch.isfinite(out).all() and out.abs().sum() > 0 and torch.isfinite(g).all()
+print("captured")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
 def test_trainer_refusals(lib):
     cfg, sp, _, _, _ = scene(n=300)
     for kw in (dict(dropout=DropoutOptions(splat_rate=1.0)), dict(dropout=DropoutOptions(sh_rate=-0.1)), dict(dropout=DropoutOptions(sh_rate=0.1, sh_group=0)),
