@@ -56,7 +56,9 @@ constexpr int kDropChunks = 4;                                     // chunks of 
 constexpr int kDropTile = kDropThreads * kDropChunks * 4;          // values per block
 
 // Every value decides for itself: a thread's four values are the four words of one generator block, so the decisions never
-// leave registers.  Chunks start on multiples of four of the whole array's numbering.
+// leave registers.  Chunks start on multiples of four of the whole array's numbering.  Bound by memory, 8 bytes a value: 135M values in
+// 172 us, 6.3 TB/s, 96 % of the copy bandwidth; the generator's ten rounds fit behind it.
+// One chunk a thread less or more: 167 (two) and 160 us (eight) where four took 157 on the same day.
 template <bool VEC>
 __global__ void __launch_bounds__(kDropThreads) dropout_values_kernel(const float* x, float* y, int64_t first, int64_t count, DropArgs a) {
     const uint64_t offset = drop_offset(a);
@@ -77,7 +79,8 @@ __global__ void __launch_bounds__(kDropThreads) dropout_values_kernel(const floa
 }
 
 // Groups of several values: the decisions of the groups that a block's tile touches are made once, one generator block per
-// four groups, and kept as one byte each in shared memory while the tile's values are on their way.
+// four groups, and kept as one byte each in shared memory while the tile's values are on their way.  45M values in groups of three: 57 us,
+// 6.3 TB/s, 96 % of the copy bandwidth; with a 64-bit place per value it was 69 us and bound by integer arithmetic.
 struct GroupArgs {
     uint32_t group, magic;
     uint32_t first_rem;        // place of the first value in its group
@@ -164,7 +167,12 @@ __device__ __forceinline__ float drop_opacity(float x, float v, bool dropped, co
     return dropped ? kDroppedLogit : (x > o.x_cap ? o.capped : fmaf(-0.6931471805599453f, l, x + o.a));
 }
 
+// Two chunks of loads in flight per thread; one took 31 + 27 us where two took 29 + 25, four 29 + 30 (forward + backward, before the
+// hardware logarithm).
 constexpr int kOpacityChunks = 2;
+
+// 8 bytes a splat forward, 12 backward.  10M splats: 20.7 and 24.6 us; ssb_dropout, which moves the forward call's bytes with a fifth of
+// its arithmetic, takes 16.6 at that size, a device copy of torch's 20.7.
 
 template <bool BWD, bool VEC>
 __global__ void __launch_bounds__(kDropThreads) dropout_opacity_kernel(const float* x, const float* v, float* out, int64_t first, int64_t count,

@@ -7,10 +7,12 @@
 namespace ssb {
 
 // ---- 4-bit rows -------------------------------------------------------------
-// A band's scale is the smallest bf16 s with 7 s >= the largest finite magnitude m of the band (zero below 2^-100, where s
-// and its multiples would lose bits, and one step smaller where 7 s would overflow); a value's code is v / s rounded to the nearest integer, ties to even, so that
-// decode(encode(v)) is within s / 2.  The quotient is not formed: q = rint(v * (1 / s)) is off by one at most next to a
-// midpoint, and the remainder v - q s, exact in one fused multiply-add (it has at most the bits of v below s), tells.
+// A band's scale is the smallest bf16 s with 7 s >= the largest finite magnitude m of the band (zero below 2^-100, where s and its
+// multiples would lose bits, and one step smaller where 7 s would overflow); a value's code is v / s rounded to the nearest
+// integer, ties to even, so that decode(encode(v)) is within s / 2.  The scale is rounded up to bf16's eight bits before the codes
+// are taken: that widens a step by less than 1/128 and makes every decoded value an exact float (eleven bits).
+// The quotient is not formed: q = rint(v * (1 / s)) is off by one at most next to a midpoint, and the remainder v - q s, exact in
+// one fused multiply-add (it has at most the bits of v below s), tells.
 __device__ __forceinline__ float row_scale(float m) {
     if (!(m >= 7.8886090522101181e-31f)) return 0.0f;                                      // 2^-100
     float s = __uint_as_float(__float_as_uint(m * (1.0f / 7.0f)) & 0xffff0000u);            // within one bf16 step of the answer
@@ -40,7 +42,9 @@ __device__ __noinline__ void encode_row_checked(const float* sh, uint32_t w[6], 
 
 // Per value: t = v / s + 8 + 1.5 2^23 rounds to the code and leaves it in the low bits of t, so a word is a sum of shifted t's less
 // a constant.  The remainder decides whether the rounding was the right one (see row_code); rows with a value next to a midpoint,
-// an infinity or a NaN -- one splat in a hundred thousand of ordinary ones -- take the checked way.
+// an infinity or a NaN -- a few splats in a hundred thousand of ordinary ones -- take the checked way.
+// Bound by memory: a block's 128 rows of values come in as 16-byte asynchronous copies, its rows leave as two 16-byte stores per
+// splat.  5M splats: 173 us for 1.06 GB (6.1 TB/s); one value at a time with a conversion to integer it was 282 us.
 __global__ void __launch_bounds__(kProjBlock) sh_rows_encode_kernel(const float* __restrict__ sh, int64_t n, uint4* __restrict__ rows) {
     __shared__ __align__(16) float sh_s[kProjBlock * kShPerSplat];
     const int64_t first = (int64_t)blockIdx.x * kProjBlock;
@@ -116,6 +120,8 @@ __device__ __forceinline__ void bulk_done() {
     if (threadIdx.x == 0) asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 
+// Bound by memory: one row per thread, the block's values leave as one bulk copy.  5M splats: 151 us behind the encoder, whose rows are
+// then partly in L2.
 __global__ void __launch_bounds__(kProjBlock) sh_rows_decode_kernel(const void* __restrict__ rows, int64_t n, float* __restrict__ sh) {
     __shared__ __align__(16) float sh_s[kProjBlock * kShPerSplat];
     const int64_t first = (int64_t)blockIdx.x * kProjBlock;
@@ -150,7 +156,9 @@ int launch_sh_rows_decode(const void* d_rows, int64_t n, float* d_values, cudaSt
 // One view of 4-bit rows (the *_row kernels) is bound by memory: a thread per splat, nothing kept, codes decoded where they are
 // multiplied.  Several views, or values in another form (the *_views kernels), are bound by arithmetic: a thread works on two
 // splats at once, 128 apart, with the coefficients in registers, and all its arithmetic is on pairs, one packed single-precision
-// instruction for two results.
+// instruction for two results.  What limits that is the register file: a packed multiply-add on three different register pairs was
+// measured at three cycles per scheduler, a scalar one at 1.9, so a pair costs less than two scalars; one splat per thread, scalar or
+// packed over coefficients, took 76 and 81 us where this form takes 64 (1M splats, 16 views, forward) and 157 against 154 backward.
 typedef float2 Pair;
 __device__ __forceinline__ Pair operator+(Pair a, Pair b) { return __fadd2_rn(a, b); }
 __device__ __forceinline__ Pair operator*(Pair a, Pair b) { return __fmul2_rn(a, b); }
@@ -298,8 +306,10 @@ __device__ __noinline__ void eval_checked(const SsbSplats sp, const float* sh, c
 }
 
 // ---- one view of 4-bit rows ----
-constexpr int kRowBlock = 128;
-constexpr int kRowBlocksPerSm = 8;
+constexpr int kRowBlock = kProjBlock;
+// 10M splats: with 8 blocks (64 registers) 121 us, 6 (79) 112, 5 (93) 121, 4 (107) 131: fewer registers cost moves, fewer blocks loads
+// under way.
+constexpr int kRowBlocksPerSm = 6;
 
 // Components of -centre of view 0 as two floats each, by the block's first three threads; a barrier follows.
 __device__ __forceinline__ void stage_centre(ViewCentre<float>& c, const float* __restrict__ viewmats) {
@@ -321,6 +331,10 @@ __device__ __forceinline__ void load_row_inputs(RowInputs& in, const char* rows,
         for (int k = 0; k < 3; ++k) in.dc[k] = dc[3 * t + k];
 }
 
+// 68 bytes a splat (row, mean, DC, value) and 280 instructions.  10M splats: 112 us, 6.1 TB/s, 93 % of the copy bandwidth, in a short
+// run; called without a pause the GPU reaches its power limit, lowers its clock to 1.7 GHz, and it is 130 us.  The blocks stay for all
+// their tiles: the camera's centre is taken once, and the next tile's loads are under way while a tile is worked on (one tile per
+// block: 137 us, 158 with the outputs staged).  Multiply-adds and the codes' offsets on pairs of coefficients: 330 instructions before.
 __global__ void __launch_bounds__(kRowBlock, kRowBlocksPerSm) sh_eval_fwd_row_kernel(SsbSplats sp, const void* __restrict__ rows, int64_t n,
                                                                                      const float* __restrict__ viewmats, int n_sh, float* __restrict__ out) {
     __shared__ ViewCentre<float> centre_s;
@@ -350,20 +364,20 @@ __global__ void __launch_bounds__(kRowBlock, kRowBlocksPerSm) sh_eval_fwd_row_ke
         const Polynomials<float> o = sh_polynomials(view_directions(centre, now.mean, d2));
 #pragma unroll
         for (int ch = 0; ch < 3; ++ch) c[ch] = kShC0 * now.dc[ch];
+        // coefficients (2k, 2k + 1) side by side; the last pair's second half is coefficient 14 again, times zero
+        const float sc[3] = {active_scale(now.r, 0, n_sh), active_scale(now.r, 1, n_sh), active_scale(now.r, 2, n_sh)};
+        Pair sum[3] = {make_float2(c[0], 0.0f), make_float2(c[1], 0.0f), make_float2(c[2], 0.0f)};
 #pragma unroll
-        for (int b = 0; b < 3; ++b) {
-            float t[3] = {0.f, 0.f, 0.f};
+        for (int j = 0; j < kNumSh; j += 2) {
+            const int j1 = j + 1 < kNumSh ? j + 1 : j;
+            const Pair f = make_float2((sh_constant(j) * code_unit(j)) * o.p[j], (sh_constant(j1) * code_unit(j1)) * o.p[j1]) *
+                           make_float2(sc[sh_band(j)], j1 > j ? sc[sh_band(j1)] : 0.0f);
 #pragma unroll
-            for (int j = 0; j < kNumSh; ++j)
-                if (sh_band(j) == b) {
-                    const float f = (sh_constant(j) * code_unit(j)) * o.p[j];
-#pragma unroll
-                    for (int ch = 0; ch < 3; ++ch) t[ch] = fmaf(f, code_of(now.r, j, ch), t[ch]);
-                }
-            const float s = active_scale(now.r, b, n_sh);
-#pragma unroll
-            for (int ch = 0; ch < 3; ++ch) c[ch] = fmaf(s, t[ch], c[ch]);
+            for (int ch = 0; ch < 3; ++ch)
+                sum[ch] = fma_(f, make_float2(code_bits(now.r, j, ch), code_bits(now.r, j1, ch)) + make_float2(code_bias(j), code_bias(j1)), sum[ch]);
         }
+#pragma unroll
+        for (int ch = 0; ch < 3; ++ch) c[ch] = sum[ch].x + sum[ch].y;
         if (mine) {
 #pragma unroll
             for (int ch = 0; ch < 3; ++ch) op[3 * threadIdx.x + ch] = c[ch];
@@ -374,6 +388,9 @@ __global__ void __launch_bounds__(kRowBlock, kRowBlocksPerSm) sh_eval_fwd_row_ke
     }
 }
 
+// 260 bytes a splat, 204 of them written.  3M splats: 121 us, 6.4 TB/s, 98 % of the copy bandwidth.  A tile's three arrays of gradients
+// are contiguous spans, written to shared memory at a stride of 45 words (no bank conflicts) and sent off as three bulk copies; with
+// direct stores it was 699 us.
 __global__ void __launch_bounds__(kRowBlock) sh_eval_bwd_row_kernel(SsbSplats sp, const void* __restrict__ rows, int64_t n, const float* __restrict__ viewmats,
                                                                     int n_sh, const float* __restrict__ v_out, SsbSplats gr, int accumulate) {
     __shared__ __align__(16) float sh_s[kRowBlock * kShPerSplat];
@@ -511,8 +528,12 @@ __device__ __forceinline__ void to_azimuthal(Pair A[16 * 3], const Pair W[kShPer
     }
 }
 
-constexpr int kFwdBlocksPerSm = 3, kBwdBlocksPerSm = 2;       // what their registers allow; the grids are this many blocks
+// What the registers allow (150 and 252 per thread); the grids are this many blocks, which walk the tiles.  Four forward blocks
+// make the compiler spill: 73 us against 64.
+constexpr int kFwdBlocksPerSm = 3, kBwdBlocksPerSm = 2;
 
+// Per (splat, view): the direction (12 operations), the azimuthal functions (7) and 45 multiply-adds.  1M splats, 16 views: 64 us;
+// 20.8M packed instructions at the three cycles of the register file are 55 us, the bytes (248 MB) 38 us.
 template <bool ROWS>
 __global__ void __launch_bounds__(kProjBlock, kFwdBlocksPerSm) sh_eval_fwd_views_kernel(SsbSplats sp, SsbShQuant shq, int64_t n, int views,
                                                                                         const float* __restrict__ viewmats, int n_sh,
@@ -606,6 +627,9 @@ __device__ __forceinline__ void fetch_grads(GradRing& ring, int slot, GradCursor
     asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
+// Per (splat, view): direction and polynomials (35 operations), 45 multiply-adds for the coefficients' gradients, 45 for the sums w_j
+// and 40 for the mean's.  The 45 gradients of both splats stay in registers over all views, so nothing is added in memory and the sum
+// has one order.  1M splats, 16 views: 154 us; 47.5M packed instructions at three cycles are 125 us, the bytes (440 MB) 67 us.
 template <bool ROWS>
 __global__ void __launch_bounds__(kProjBlock, kBwdBlocksPerSm) sh_eval_bwd_views_kernel(SsbSplats sp, SsbShQuant shq, int64_t n, int views,
                                                                                         const float* __restrict__ viewmats, int n_sh,

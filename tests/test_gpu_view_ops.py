@@ -455,3 +455,115 @@ def test_eval_on_another_stream_and_in_a_graph(lib):
     torch.cuda.synchronize()
     c2 = dict(c, sh=-c["sh"])
     assert torch.equal(out, run_fwd(lib, c2, sources(lib, c2["sh"], 4)))
+
+
+# ---- beyond 32 bits, and several calls at once -----------------------------------------------------------------------
+
+def room(nbytes):
+    free, _ = torch.cuda.mem_get_info()
+    return free > nbytes + (4 << 30)
+
+
+def test_dropout_of_more_than_2_31_values(lib):
+    n = 2 ** 31 + 4099
+    if not room(4 * n):
+        pytest.skip("not enough device memory")
+    t = torch.ones(n, device=DEV)
+    for group in (1, 3):
+        t.fill_(1.0)
+        d = L.dropout_struct(0.5, SEED, OFFSET)
+        L.check(lib.ssb_dropout(L.ptr(t), 5, n, group, C.byref(d), L.ptr(t), None))
+        for a in (0, 2 ** 31 - 2000, n - 5000):
+            want = O.dropped(5 + a, 5000 if a else 3000, group, 0.5, SEED, OFFSET)
+            assert np.array_equal(t[a:a + want.size].cpu().numpy() == 0, want), (group, a)
+    d = L.dropout_struct(0.25, SEED, OFFSET)
+    t.fill_(0.5)
+    L.check(lib.ssb_dropout_opacities(L.ptr(t), 5, n, C.byref(d), L.ptr(t), None))
+    a = n - 5000
+    assert np.array_equal(t[a:].cpu().numpy() == O.DROPPED, O.dropped(5 + a, 5000, 1, 0.25, SEED, OFFSET))
+
+
+def test_rows_and_values_of_more_than_2_31_elements(lib):
+    n = 2 ** 31 // 45 + 1001                                # values pass 2^31
+    if not room(n * (180 + 32)):
+        pytest.skip("not enough device memory")
+    sh = torch.zeros(n, 15, 3, device=DEV)
+    tail = row_inputs(1000, 3)
+    sh[-1000:] = dev(tail)
+    rows = encode(lib, sh)
+    q, s = O.encode_rows(tail)
+    assert np.array_equal(rows[-1000:].cpu().numpy(), O.pack_rows(q, s))
+    L.check(lib.ssb_quant_decode(L.ptr(rows), None, n * 45, 4, L.ptr(sh), None))
+    assert np.array_equal(sh[-1000:].cpu().numpy(), O.row_values(q, s).astype(np.float32)) and not sh[:1000].any()
+
+
+def test_eval_of_more_than_2_31_outputs_and_gradients(lib):
+    n, views = 45_000_003, 17                               # 3 n views and 45 n pass 2^31
+    if not room(n * (32 + 24 + 12 * views + 204)):
+        pytest.skip("not enough device memory")
+    k = 700
+    c = eval_case(k, views)
+    rows = torch.zeros(n, 32, dtype=torch.uint8, device=DEV)
+    means, dc = torch.ones(n, 3, device=DEV), torch.zeros(n, 3, device=DEV)
+    rows[-k:] = encode(lib, dev(c["sh"]))
+    means[-k:], dc[-k:] = dev(c["means"]), dev(c["dc"])
+    vm = dev(c["vm"])
+    s = L.splats_struct(dict(means=means, features_dc=dc))
+    cams = L.cameras_struct(vm, vm, 1, 1)
+    shq = L.shq_struct(rows, None, 4, 0)
+    out = torch.empty(views, n, 3, device=DEV)
+    vals = O.row_values(*O.encode_rows(c["sh"]))
+    want, tol = O.sh_eval(c["means"], c["dc"], vals, c["vm"])
+    L.check(lib.ssb_sh_eval_fwd(C.byref(s), C.byref(shq), n, C.byref(cams), L.ptr(out), None))
+    torch.cuda.synchronize()
+    within(out[:, -k:], want, tol)
+    out.zero_()                                             # the gradients' turn, in the same buffer
+    out[:, -k:] = dev(c["v"])
+    gm, gd, gs = torch.empty(n, 3, device=DEV), torch.empty(n, 3, device=DEV), torch.empty(n, 45, device=DEV)
+    g = L.splats_struct(dict(means=gm, features_dc=gd, features_sh=gs))
+    (wm, wd, ws), (tm, td, ts) = O.sh_eval_bwd(c["means"], vals, c["vm"], c["v"])
+    L.check(lib.ssb_sh_eval_bwd(C.byref(s), C.byref(shq), n, C.byref(cams), L.ptr(out), C.byref(g), 0, None))
+    torch.cuda.synchronize()
+    within(gm[-k:], wm, tm); within(gd[-k:], wd, td); within(gs[-k:].reshape(k, 15, 3), ws, ts)
+    assert not gs[:1000].any() and not gm[:1000].any()
+    one = L.cameras_struct(vm, vm, 1, 1, count=1)           # and the kernels of one view
+    want1, tol1 = O.sh_eval(c["means"], c["dc"], vals, c["vm"][:1])
+    res = torch.empty(n, 3, device=DEV)
+    L.check(lib.ssb_sh_eval_fwd(C.byref(s), C.byref(shq), n, C.byref(one), L.ptr(res), None))
+    L.check(lib.ssb_sh_eval_bwd(C.byref(s), C.byref(shq), n, C.byref(one), L.ptr(out), C.byref(g), 0, None))
+    torch.cuda.synchronize()
+    within(res[-k:], want1[0], tol1[0])
+    (wm, wd, ws), (tm, td, ts) = O.sh_eval_bwd(c["means"], vals, c["vm"][:1], c["v"][:1])
+    within(gm[-k:], wm, tm); within(gs[-k:].reshape(k, 15, 3), ws, ts)
+
+
+def test_calls_on_several_streams_at_once_and_repeated_calls_agree(lib):
+    c = eval_case(60_000, 5)
+    src = sources(lib, c["sh"], 4)
+    m, dc, vm, v, sh = dev(c["means"]), dev(c["dc"]), dev(c["vm"]), dev(c["v"]), dev(c["sh"])
+    sp = L.splats_struct(dict(means=m, features_dc=dc))
+    cams = L.cameras_struct(vm, vm, 1, 1)
+    d = L.dropout_struct(0.3, 1, 2)
+    n = 60_000
+
+    def work(stream):
+        out, gm, gs = torch.empty(5, n, 3, device=DEV), torch.empty(n, 3, device=DEV), torch.empty(n, 45, device=DEV)
+        y, rows = torch.empty(n * 45, device=DEV), torch.empty(n, 32, dtype=torch.uint8, device=DEV)
+        g = L.splats_struct(dict(means=gm, features_sh=gs))
+        torch.cuda.synchronize()
+        st = C.c_void_p(stream.cuda_stream)
+
+        def go():
+            L.check(lib.ssb_dropout(L.ptr(sh), 0, n * 45, 3, C.byref(d), L.ptr(y), st))
+            L.check(lib.ssb_quant_encode(L.ptr(y), n * 45, 4, L.ptr(rows), None, st))
+            q = L.shq_struct(rows, None, 4, 0)
+            L.check(lib.ssb_sh_eval_fwd(C.byref(sp), C.byref(q), n, C.byref(cams), L.ptr(out), st))
+            L.check(lib.ssb_sh_eval_bwd(C.byref(sp), C.byref(q), n, C.byref(cams), L.ptr(v), C.byref(g), 0, st))
+        return go, (out, gm, gs, y, rows)
+    jobs = [work(torch.cuda.Stream()) for _ in range(3)]
+    for _ in range(4):
+        for go, _ in jobs:
+            go()
+    torch.cuda.synchronize()
+    for _, res in jobs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(jobs[0][1], res))

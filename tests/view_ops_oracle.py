@@ -154,9 +154,10 @@ def directions(means, viewmat):
 
 
 # Errors of an fp32 evaluation in units of U.  A component of the difference mean - centre is off by 2 (two additions), the
-# squared length by 8, the reciprocal root (one Newton step on a 2-ulp start) by 4 + 8/2, a unit component by 12 in all.  With
-# the largest magnitudes of the monomials that makes, per band: the basis function; its largest value and the error and the
-# largest value of a component of its gradient.
+# squared length by 8, the reciprocal root (2 ulps are 4 U) by 4 + 8/2, a unit component by 12 in all.  With the largest magnitudes
+# of the monomials that makes, per band: the basis function (summed by itself, or with its monomials' coefficients gathered first:
+# b = c z^2 - c/3 at z^2 = 1/3 loses no more than 2 c/3 times the roundings that follow, within the 27); its largest value and the
+# error and the largest value of a component of its gradient.
 BASIS_ERR = (7.0, 27.0, 100.0)
 GRAD_ERR = (10.0, 40.0, 240.0)
 GRAD_MAX = (0.49, 2.2, 7.0)
