@@ -44,7 +44,7 @@ __device__ __noinline__ void encode_row_checked(const float* sh, uint32_t w[6], 
 // a constant.  The remainder decides whether the rounding was the right one (see row_code); rows with a value next to a midpoint,
 // an infinity or a NaN -- a few splats in a hundred thousand of ordinary ones -- take the checked way.
 // Bound by memory: a block's 128 rows of values come in as 16-byte asynchronous copies, its rows leave as two 16-byte stores per
-// splat.  5M splats: 173 us for 1.06 GB (6.1 TB/s); one value at a time with a conversion to integer it was 282 us.
+// splat.  5M splats: 156 us for 1.06 GB, at the copy bandwidth; one value at a time with a conversion to integer it was 282 us.
 __global__ void __launch_bounds__(kProjBlock) sh_rows_encode_kernel(const float* __restrict__ sh, int64_t n, uint4* __restrict__ rows) {
     __shared__ __align__(16) float sh_s[kProjBlock * kShPerSplat];
     const int64_t first = (int64_t)blockIdx.x * kProjBlock;
@@ -120,8 +120,7 @@ __device__ __forceinline__ void bulk_done() {
     if (threadIdx.x == 0) asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 
-// Bound by memory: one row per thread, the block's values leave as one bulk copy.  5M splats: 151 us behind the encoder, whose rows are
-// then partly in L2.
+// Bound by memory: one row per thread, the block's values leave as one bulk copy.  5M splats: 160 us for 1.06 GB.
 __global__ void __launch_bounds__(kProjBlock) sh_rows_decode_kernel(const void* __restrict__ rows, int64_t n, float* __restrict__ sh) {
     __shared__ __align__(16) float sh_s[kProjBlock * kShPerSplat];
     const int64_t first = (int64_t)blockIdx.x * kProjBlock;
