@@ -423,6 +423,37 @@ def test_eval_far_from_the_origin_and_at_the_camera(lib):
     within(g["means"], gm, tm); within(g["features_sh"], gs, ts)
 
 
+@pytest.mark.parametrize("fmt", [4, 32])
+@pytest.mark.parametrize("views", [1, 2, 35])
+def test_eval_of_degenerate_splats_beside_ordinary_ones(lib, fmt, views):
+    """Splats at a camera's centre, next to it and out of range of a float's square, each sharing a thread or a warp with ordinary
+    ones, and non-finite positions, which concern only their own splat."""
+    n = 700
+    c = eval_case(n, views, seed=11)
+    vm = c["vm"].reshape(views, 4, 4)
+    vm[0, :3, :3], vm[0, :3, 3] = np.eye(3), (-1.0, -2.0, -4.0)              # centre (1, 2, 4), exactly
+    bad = np.arange(3, n, 61)
+    odd = [(1, 2, 4), (1, 2, 4 + 2.0 ** -20), (1e20, 2, 3), (-3e30, 1e30, 4), (1, 2 + 2.0 ** -21, 4), (1e16, 1e16, 1e16)]
+    for k, i in enumerate(bad):
+        c["means"][i] = odd[k % len(odd)]
+    broken = np.array([130, 259, 600])
+    c["means"][broken[0]] = np.nan; c["means"][broken[1], 1] = np.inf; c["means"][broken[2], 2] = -np.inf
+    fine = np.setdiff1d(np.arange(n), broken)
+    src = sources(lib, c["sh"], fmt)
+    means = c["means"].copy()
+    means[broken] = 0
+    want, tol = O.sh_eval(means, c["dc"], src[2], c["vm"])
+    got = run_fwd(lib, c, src)
+    within(got[:, torch.from_numpy(fine).to(DEV)], want[:, fine], tol[:, fine])
+    assert torch.isnan(got[:, torch.from_numpy(broken).to(DEV)]).all()
+    (gm, gd, gs), (tm, td, ts) = O.sh_eval_bwd(means, src[2], c["vm"], c["v"])
+    g = run_bwd(lib, c, src)
+    pick = lambda t, w: t.view(n, w)[torch.from_numpy(fine).to(DEV)]
+    within(pick(g["means"], 3), gm[fine], tm[fine]); within(pick(g["features_dc"], 3), gd[fine], td[fine])
+    within(pick(g["features_sh"], 45).reshape(-1, 15, 3), gs[fine], ts[fine])
+    assert torch.isnan(g["means"].view(n, 3)[torch.from_numpy(broken).to(DEV)]).any(1).all()
+
+
 def test_eval_on_another_stream_and_in_a_graph(lib):
     c = eval_case(1000, 4)
     src = sources(lib, c["sh"], 4)

@@ -73,8 +73,13 @@ def test_projection_of_rows_equals_projection_of_their_values(lib, n, model, deg
         cnt = torch.zeros(1, dtype=torch.int64, device=DEV)
         L.check(lib.ssb_project_fwd_packed(C.byref(struct), q, n, C.byref(cams), L.ptr(ws), ws.numel(), L.ptr(paabb), L.ptr(pdep), None, L.ptr(prec),
                                            L.ptr(ci), L.ptr(gi), views * n, L.ptr(cnt), None, None))
+        pgrads = {k: torch.zeros_like(v) for k, v in t.items()}
+        gp = L.splats_struct(pgrads)
+        ws2 = torch.zeros(lib.ssb_project_bwd_packed_workspace_bytes(n, views), dtype=torch.uint8, device=DEV)
+        L.check(lib.ssb_project_bwd_packed(C.byref(struct), q, n, C.byref(cams), L.ptr(paabb), L.ptr(v_rec), L.ptr(ci), L.ptr(gi), L.ptr(cnt), views * n,
+                                           L.ptr(ws2), ws2.numel(), C.byref(gp), 0, None))
         torch.cuda.synchronize()
-        outs.append([aabb, depths, rec, *grads.values(), *single.values(), paabb, pdep, prec, cnt])
+        outs.append([aabb, depths, rec, *grads.values(), *single.values(), *pgrads.values(), paabb, pdep, prec, cnt])
     assert n == 1 or int(outs[0][-1]) > n // 4
     for a, b in zip(*outs):
         assert torch.equal(a.reshape(-1).view(torch.int32 if a.dtype == torch.float32 else a.dtype), b.reshape(-1).view(torch.int32 if b.dtype == torch.float32 else b.dtype))
