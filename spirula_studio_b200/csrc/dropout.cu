@@ -8,19 +8,18 @@ namespace ssb {
 constexpr float kDroppedLogit = SSB_DROPPED_LOGIT;
 
 struct DropArgs {
-    uint32_t key0, key1;
+    uint32_t k0[10], k1[10];       // the rounds' keys (added up in the kernel instead: 57 and 172 us where these take 56 and 169)
     uint64_t offset;
     const uint64_t* d_offset;
     uint32_t threshold;        // a group is dropped when its word is below it
     float scale;               // 1 / (1 - rate)
 };
 
-__device__ __forceinline__ uint4 philox4x32_10(uint4 c, uint32_t k0, uint32_t k1) {
+__device__ __forceinline__ uint4 philox4x32_10(uint4 c, const uint32_t* k0, const uint32_t* k1) {
 #pragma unroll
     for (int r = 0; r < 10; ++r) {
         const uint64_t p = (uint64_t)c.x * 0xD2511F53u, q = (uint64_t)c.z * 0xCD9E8D57u;
-        c = make_uint4((uint32_t)(q >> 32) ^ c.y ^ k0, (uint32_t)q, (uint32_t)(p >> 32) ^ c.w ^ k1, (uint32_t)p);
-        k0 += 0x9E3779B9u; k1 += 0xBB67AE85u;
+        c = make_uint4((uint32_t)(q >> 32) ^ c.y ^ k0[r], (uint32_t)q, (uint32_t)(p >> 32) ^ c.w ^ k1[r], (uint32_t)p);
     }
     return c;
 }
@@ -29,7 +28,7 @@ __device__ __forceinline__ uint64_t drop_offset(const DropArgs& a) { return a.of
 
 // The four words of block b: the decisions of groups 4b .. 4b + 3.
 __device__ __forceinline__ uint4 drop_words(const DropArgs& a, uint64_t offset, uint64_t block) {
-    return philox4x32_10(make_uint4((uint32_t)block, (uint32_t)(block >> 32), (uint32_t)offset, (uint32_t)(offset >> 32)), a.key0, a.key1);
+    return philox4x32_10(make_uint4((uint32_t)block, (uint32_t)(block >> 32), (uint32_t)offset, (uint32_t)(offset >> 32)), a.k0, a.k1);
 }
 // Four consecutive values at p[i], of which only those with 0 <= i + k < count exist.  VEC: p + i is 16-byte aligned.
 template <bool VEC>
@@ -57,7 +56,7 @@ constexpr int kDropTile = kDropThreads * kDropChunks * 4;          // values per
 
 // Every value decides for itself: a thread's four values are the four words of one generator block, so the decisions never
 // leave registers.  Chunks start on multiples of four of the whole array's numbering.  Bound by memory, 8 bytes a value: 135M values in
-// 172 us, 6.3 TB/s, 96 % of the copy bandwidth; the generator's ten rounds fit behind it.
+// 169 us, 6.4 TB/s, 98 % of the copy bandwidth; the generator's ten rounds fit behind it.
 // One chunk a thread less or more: 167 (two) and 160 us (eight) where four took 157 on the same day.
 template <bool VEC>
 __global__ void __launch_bounds__(kDropThreads) dropout_values_kernel(const float* x, float* y, int64_t first, int64_t count, DropArgs a) {
@@ -79,8 +78,8 @@ __global__ void __launch_bounds__(kDropThreads) dropout_values_kernel(const floa
 }
 
 // Groups of several values: the decisions of the groups that a block's tile touches are made once, one generator block per
-// four groups, and kept as one byte each in shared memory while the tile's values are on their way.  45M values in groups of three: 57 us,
-// 6.3 TB/s, 96 % of the copy bandwidth; with a 64-bit place per value it was 69 us and bound by integer arithmetic.
+// four groups, and kept as one byte each in shared memory while the tile's values are on their way.  45M values in groups of three: 56 us,
+// 6.4 TB/s, 98 % of the copy bandwidth; with a 64-bit place per value it was 69 us and bound by integer arithmetic.
 struct GroupArgs {
     uint32_t group, magic;
     uint32_t first_rem;        // place of the first value in its group
@@ -171,8 +170,8 @@ __device__ __forceinline__ float drop_opacity(float x, float v, bool dropped, co
 // hardware logarithm).
 constexpr int kOpacityChunks = 2;
 
-// 8 bytes a splat forward, 12 backward.  10M splats: 20.7 and 24.6 us; ssb_dropout, which moves the forward call's bytes with a fifth of
-// its arithmetic, takes 16.6 at that size, a device copy of torch's 20.7.
+// 8 bytes a splat forward, 12 backward.  10M splats: 20.8 to 22.8 and 24.0 us; ssb_dropout, which moves the forward call's bytes with a third of
+// its arithmetic, takes 16.0 at that size, a device copy of torch's 20.7.
 
 template <bool BWD, bool VEC>
 __global__ void __launch_bounds__(kDropThreads) dropout_opacity_kernel(const float* x, const float* v, float* out, int64_t first, int64_t count,
@@ -203,7 +202,10 @@ static int drop_args(const SsbDropout* d, const char* who, DropArgs* a) {
     SSB_REQUIRE(d->rate >= 0.0f && d->rate < 1.0f, "%s: the rate must be in [0, 1) (got %g)", who, (double)d->rate);
     SSB_REQUIRE(d->reserved == 0, "%s: reserved must be 0", who);
     SSB_REQUIRE(((uintptr_t)d->d_offset & 7) == 0, "%s: d_offset must be 8-byte aligned", who);
-    a->key0 = (uint32_t)d->seed; a->key1 = (uint32_t)(d->seed >> 32);
+    for (int r = 0; r < 10; ++r) {
+        a->k0[r] = (uint32_t)d->seed + (uint32_t)r * 0x9E3779B9u;
+        a->k1[r] = (uint32_t)(d->seed >> 32) + (uint32_t)r * 0xBB67AE85u;
+    }
     a->offset = d->offset;
     a->d_offset = d->d_offset;
     a->threshold = (uint32_t)floor((double)d->rate * 4294967296.0);
