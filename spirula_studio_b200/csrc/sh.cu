@@ -152,8 +152,8 @@ int launch_sh_rows_decode(const void* d_rows, int64_t n, float* d_values, cudaSt
 // The basis functions are taken as polynomials p_j of the direction without their constants k_j (b_j = k_j p_j); the constants go
 // into the coefficients or into their gradients, once per splat.
 //
-// One view of 4-bit rows (the *_row kernels) is bound by memory: a thread per splat, nothing kept, codes decoded where they are
-// multiplied.  Several views, or values in another form (the *_views kernels), are bound by arithmetic: a thread works on two
+// One view is bound by memory: a thread per splat, nothing kept, codes decoded where they are multiplied.  Several views (the *_views
+// kernels) are bound by arithmetic: a thread works on two
 // splats at once, 128 apart, with the coefficients in registers, and all its arithmetic is on pairs, one packed single-precision
 // instruction for two results.  What limits that is the register file: a packed multiply-add on three different register pairs was
 // measured at three cycles per scheduler, a scalar one at 1.9, so a pair costs less than two scalars; one splat per thread, scalar or
@@ -304,7 +304,7 @@ __device__ __noinline__ void eval_checked(const SsbSplats sp, const float* sh, c
     }
 }
 
-// ---- one view of 4-bit rows ----
+// ---- one view ----
 constexpr int kRowBlock = kProjBlock;
 // 10M splats: with 8 blocks (64 registers) 121 us, 6 (79) 112, 5 (93) 121, 4 (107) 131: fewer registers cost moves, fewer blocks loads
 // under way.
@@ -387,43 +387,84 @@ __global__ void __launch_bounds__(kRowBlock, kRowBlocksPerSm) sh_eval_fwd_row_ke
     }
 }
 
-// 260 bytes a splat, 204 of them written.  3M splats: 121 us, 6.4 TB/s, 98 % of the copy bandwidth.  A tile's three arrays of gradients
-// are contiguous spans, written to shared memory at a stride of 45 words (no bank conflicts) and sent off as three bulk copies; with
-// direct stores it was 699 us.
-__global__ void __launch_bounds__(kRowBlock) sh_eval_bwd_row_kernel(SsbSplats sp, const void* __restrict__ rows, int64_t n, const float* __restrict__ viewmats,
-                                                                    int n_sh, const float* __restrict__ v_out, SsbSplats gr, int accumulate) {
+// The same for values in another form: a block's 128 splats' values are staged in shared memory as the projection does.  3M splats: fp32
+// 99 us, the copy bandwidth; 16-bit codes 134 and 8-bit ones 148, bound by decoding.  On the kernel of several views: 109, 196, 177.
+__global__ void __launch_bounds__(kRowBlock) sh_eval_fwd_staged_kernel(SsbSplats sp, SsbShQuant shq, int64_t n, const float* __restrict__ viewmats, int n_sh,
+                                                                       float* __restrict__ out) {
+    __shared__ __align__(16) float sh_s[kRowBlock * kShPerSplat];
+    __shared__ __align__(16) unsigned char raw_s[kShRawBytes];
+    __shared__ ViewCentre<float> centre_s;
+    const int64_t first = (int64_t)blockIdx.x * kRowBlock, i = first + threadIdx.x, il = min(i, n - 1);
+    const float mean[3] = {sp.means[3 * il], sp.means[3 * il + 1], sp.means[3 * il + 2]};
+    float c[3] = {0.f, 0.f, 0.f};
+    if (sp.features_dc) { c[0] = sp.features_dc[3 * il]; c[1] = sp.features_dc[3 * il + 1]; c[2] = sp.features_dc[3 * il + 2]; }
+    stage_centre(centre_s, viewmats);
+    stage_sh(sh_s, raw_s, sp.features_sh, shq.packed, shq.bounds, shq.bits, shq.bounds_stride, first, n);
+    __syncthreads();
+    if (i >= n) return;
+    const float* W = sh_s + threadIdx.x * kShPerSplat;
+    float d2;
+    const Polynomials<float> o = sh_polynomials(view_directions(centre_s, mean, d2));
+#pragma unroll
+    for (int ch = 0; ch < 3; ++ch) c[ch] *= kShC0;
+#pragma unroll
+    for (int j = 0; j < kNumSh; ++j)
+        if (j < n_sh) {
+            const float f = sh_constant(j) * o.p[j];
+#pragma unroll
+            for (int ch = 0; ch < 3; ++ch) c[ch] = fmaf(f, W[3 * j + ch], c[ch]);
+        }
+#pragma unroll
+    for (int ch = 0; ch < 3; ++ch) out[3 * i + ch] = c[ch];
+    if (!(d2 > kSquareMin && d2 < kSquareMax)) eval_checked(sp, W, nullptr, i, n, 1, viewmats, n_sh, out, nullptr, nullptr);
+}
+
+// 260 bytes a splat from 4-bit rows, 204 of them written.  3M splats: 121 us, 6.4 TB/s, 98 % of the copy bandwidth.  A tile's three
+// arrays of gradients are contiguous spans, written to shared memory at a stride of 45 words (no bank conflicts) and sent off as three
+// bulk copies; with direct stores it was 699 us.  Values in another form are staged in the span that their gradients leave from: fp32 183 us,
+// 16-bit codes 211, 8-bit 217 (266, 389, 343 on the kernel of several views).
+template <bool ROWS>
+__global__ void __launch_bounds__(kRowBlock) sh_eval_bwd_one_kernel(SsbSplats sp, SsbShQuant shq, int64_t n, const float* __restrict__ viewmats, int n_sh,
+                                                                    const float* __restrict__ v_out, SsbSplats gr, int accumulate) {
     __shared__ __align__(16) float sh_s[kRowBlock * kShPerSplat];
     __shared__ __align__(16) float mean_s[kRowBlock * 3];
     __shared__ __align__(16) float dc_s[kRowBlock * 3];
+    __shared__ __align__(16) unsigned char raw_s[ROWS ? 16 : kShRawBytes];
     __shared__ ViewCentre<float> centre_s;
     const int64_t first = (int64_t)blockIdx.x * kRowBlock, i = first + threadIdx.x, il = min(i, n - 1);
+    const void* rows = ROWS && n_sh > 0 ? shq.packed : nullptr;
     ShRow r = {};
-    if (n_sh > 0) r = load_sh_row(rows, il);
+    if (rows) r = load_sh_row(rows, il);
     const float mean[3] = {sp.means[3 * il], sp.means[3 * il + 1], sp.means[3 * il + 2]};
     const float g[3] = {v_out[3 * il], v_out[3 * il + 1], v_out[3 * il + 2]};
     stage_centre(centre_s, viewmats);
+    if (!ROWS) stage_sh(sh_s, raw_s, sp.features_sh, shq.packed, shq.bounds, shq.bits, shq.bounds_stride, first, n);
     __syncthreads();
+    float* W = sh_s + threadIdx.x * kShPerSplat;              // the splat's values, then their gradients
     float d2, w[kNumSh], vm[3];
     const Directions<float> d = view_directions(centre_s, mean, d2);
     const Polynomials<float> o = sh_polynomials(d);
+    const bool checked = !(d2 > kSquareMin && d2 < kSquareMax) && i < n;
+    float e[6 + kShPerSplat];
+    if (checked) eval_checked(sp, W, rows, i, n, 1, viewmats, n_sh, nullptr, v_out, e);
 #pragma unroll
     for (int j = 0; j < kNumSh; ++j) {
-        float t = code_of(r, j, 0) * g[0];
-        t = fmaf(code_of(r, j, 1), g[1], t);
-        t = fmaf(code_of(r, j, 2), g[2], t);
         const bool active = n_sh > (sh_band(j) + 1) * (sh_band(j) + 1) - 1;
-        w[j] = active ? ((sh_grad_constant(j) * code_unit(j)) * sh_row_scale(r, sh_band(j))) * t : 0.0f;
+        if (ROWS) {
+            const float t = fmaf(code_of(r, j, 2), g[2], fmaf(code_of(r, j, 1), g[1], code_of(r, j, 0) * g[0]));
+            w[j] = active ? ((sh_grad_constant(j) * code_unit(j)) * sh_row_scale(r, sh_band(j))) * t : 0.0f;
+        } else {
+            w[j] = active ? sh_grad_constant(j) * fmaf(W[3 * j + 2], g[2], fmaf(W[3 * j + 1], g[1], W[3 * j] * g[0])) : 0.0f;
+        }
 #pragma unroll
-        for (int ch = 0; ch < 3; ++ch) sh_s[threadIdx.x * kShPerSplat + 3 * j + ch] = active ? sh_constant(j) * o.p[j] * g[ch] : 0.0f;
+        for (int ch = 0; ch < 3; ++ch) W[3 * j + ch] = active ? sh_constant(j) * o.p[j] * g[ch] : 0.0f;
     }
     sh_polynomials_vjp(d, o, w, vm);
 #pragma unroll
     for (int k = 0; k < 3; ++k) { mean_s[3 * threadIdx.x + k] = vm[k] * d.inv; dc_s[3 * threadIdx.x + k] = kShC0 * g[k]; }
-    if (!(d2 > kSquareMin && d2 < kSquareMax)) {
-        float e[6 + kShPerSplat];
-        eval_checked(sp, nullptr, n_sh ? rows : nullptr, il, n, 1, viewmats, n_sh, nullptr, v_out, e);
+    if (checked) {
         for (int k = 0; k < 3; ++k) { mean_s[3 * threadIdx.x + k] = e[k]; dc_s[3 * threadIdx.x + k] = e[3 + k]; }
-        for (int k = 0; k < kShPerSplat; ++k) sh_s[threadIdx.x * kShPerSplat + k] = e[6 + k];
+        for (int k = 0; k < kShPerSplat; ++k) W[k] = e[6 + k];
     }
     span_written();
     __syncthreads();
@@ -434,7 +475,7 @@ __global__ void __launch_bounds__(kRowBlock) sh_eval_bwd_row_kernel(SsbSplats sp
     bulk_done();
 }
 
-// ---- several views, or values in another form ----
+// ---- several views ----
 constexpr int kEvalTile = 2 * kProjBlock;      // splats per block and step
 constexpr int kCentreChunk = 32;               // views whose centres a block keeps at a time
 constexpr int kEvalShBytes = kEvalTile * kShPerSplat * (int)sizeof(float);
@@ -761,8 +802,11 @@ int ssb_sh_eval_fwd(const SsbSplats* splats, const SsbShQuant* shq, int64_t n, c
     SSB_REQUIRE(d_values && ((uintptr_t)d_values & 3) == 0, "ssb_sh_eval_fwd: d_values is NULL or not on a 4-byte boundary");
     cudaStream_t st = (cudaStream_t)stream;
     const bool rows = q.bits == 4 || n_sh == 0;
+    const unsigned tiles = (unsigned)ceil_div(n, kRowBlock);
     if (rows && cams->count == 1) {
-        sh_eval_fwd_row_kernel<<<(unsigned)std::min<int64_t>(ceil_div(n, kRowBlock), 148 * kRowBlocksPerSm), kRowBlock, 0, st>>>(*splats, q.packed, n, cams->d_viewmats, n_sh, d_values);
+        sh_eval_fwd_row_kernel<<<std::min(tiles, 148u * kRowBlocksPerSm), kRowBlock, 0, st>>>(*splats, q.packed, n, cams->d_viewmats, n_sh, d_values);
+    } else if (cams->count == 1) {
+        sh_eval_fwd_staged_kernel<<<tiles, kRowBlock, 0, st>>>(*splats, q, n, cams->d_viewmats, n_sh, d_values);
     } else {
         const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(n, kEvalTile), 148 * kFwdBlocksPerSm);
         constexpr int smem = kEvalShBytes + kShRawBytes;
@@ -789,8 +833,10 @@ int ssb_sh_eval_bwd(const SsbSplats* splats, const SsbShQuant* shq, int64_t n, c
                 "ssb_sh_eval_bwd: arrays must lie on 4-byte boundaries");
     cudaStream_t st = (cudaStream_t)stream;
     const bool rows = q.bits == 4 || n_sh == 0;
-    if (rows && cams->count == 1) {
-        sh_eval_bwd_row_kernel<<<(unsigned)ceil_div(n, kRowBlock), kRowBlock, 0, st>>>(*splats, q.packed, n, cams->d_viewmats, n_sh, d_v_values, *grads, accumulate);
+    if (cams->count == 1) {
+        const unsigned tiles = (unsigned)ceil_div(n, kRowBlock);
+        if (rows) sh_eval_bwd_one_kernel<true><<<tiles, kRowBlock, 0, st>>>(*splats, q, n, cams->d_viewmats, n_sh, d_v_values, *grads, accumulate);
+        else sh_eval_bwd_one_kernel<false><<<tiles, kRowBlock, 0, st>>>(*splats, q, n, cams->d_viewmats, n_sh, d_v_values, *grads, accumulate);
     } else {
         const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(n, kEvalTile), 148 * kBwdBlocksPerSm);
         const void* kernel = rows ? (const void*)sh_eval_bwd_views_kernel<true> : (const void*)sh_eval_bwd_views_kernel<false>;
