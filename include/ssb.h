@@ -185,7 +185,7 @@ int ssb_project_bwd(const SsbSplats* splats, const SsbShQuant* shq, int64_t n,
  * Of `splats`, means, features_dc (NULL: zeros) and features_sh (when shq names no codes) are read; of `cams`, d_viewmats,
  * count and sh_degree_plus1.  A splat at the camera's centre has no direction: its value is the features_dc term.
  * ssb_sh_eval_bwd: gradients of means, features_dc and features_sh (the coefficients' values, whatever they are stored in), summed
- * over the views in view order; an array that is NULL in `grads` is not wanted.  accumulate != 0 adds to the arrays.  Coefficients
+ * over the views in an order that depends on the sizes only; an array that is NULL in `grads` is not wanted.  accumulate != 0 adds to the arrays.  Coefficients
  * above the active degree get zero. */
 int ssb_sh_eval_fwd(const SsbSplats* splats, const SsbShQuant* shq, int64_t n, const SsbCameras* cams, float* d_values, void* stream);
 int ssb_sh_eval_bwd(const SsbSplats* splats, const SsbShQuant* shq, int64_t n, const SsbCameras* cams, const float* d_v_values,
@@ -564,9 +564,9 @@ int ssb_adam_step_sh_quantized_ex(float* d_grad, uint8_t* d_optim_packed, float*
 /* QuantizedTensor<BITS,256>::encode_v / decode_v over whole buffers
  * (src/core/Tensor.h:1366-1393); bounds = float2 per 256 cells.
  * bits = 4: the 32-byte rows of SsbShQuant, numel = 45 * splats, d_bounds is not used (NULL).  A band's scale is the smallest bf16
- * number s with 7 s >= m, m the largest finite magnitude of the band (0 when m < 2^-100; one step
- * smaller where 7 s would overflow), and a value's code is value / s rounded
- * to the nearest integer, ties to even, at most 7 in magnitude: NaN becomes 0 and an infinity +-7.  Decoding is exact. */
+ * number s with 7 s >= m, m the largest finite magnitude of the band (0 when m < 2^-100; one step smaller where 7 s would
+ * overflow), and a value's code is value / s rounded to the nearest integer, ties to even, at most 7 in magnitude: NaN becomes 0
+ * and an infinity +-7.  Decoding is exact. */
 int ssb_quant_encode(const float* d_values, int64_t numel, int32_t bits, void* d_packed, float* d_bounds, void* stream);
 int ssb_quant_decode(const void* d_packed, const float* d_bounds, int64_t numel, int32_t bits, float* d_values, void* stream);
 

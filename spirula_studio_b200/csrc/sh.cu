@@ -3,6 +3,7 @@
 #include "sh_device.cuh"
 
 #include <algorithm>
+#include <cooperative_groups.h>
 
 namespace ssb {
 
@@ -497,6 +498,14 @@ __device__ __forceinline__ void stage_tile(float* sh_s, unsigned char* raw_s, co
     __syncthreads();
 }
 
+// With few splats and many views the views are split over the grid's second dimension: block (., y) takes its share of them, which
+// is as if it had been given that many views and the arrays from its first one on.
+__device__ __forceinline__ int64_t share_of_views(int& views) {
+    const int from = (int)((int64_t)views * blockIdx.y / gridDim.y), to = (int)((int64_t)views * (blockIdx.y + 1) / gridDim.y);
+    views = to - from;
+    return from;
+}
+
 // A tile's inputs travel to shared memory while the tile before is worked on: each thread copies and reads its own two splats', so
 // no barrier is needed.
 struct TileInputs { uint4 row[4][kProjBlock]; Pair mean[3][kProjBlock], dc[3][kProjBlock]; };
@@ -510,8 +519,10 @@ __device__ __forceinline__ void fetch_pairs(const Pair* dst, const float* __rest
 }
 template <bool ROWS>
 __device__ __forceinline__ void fetch_inputs(TileInputs& in, const SsbSplats& sp, bool want_dc, const void* __restrict__ rows, int n_sh, int64_t first, int64_t n) {
-    if (first < n) {
-        const int64_t l0 = min(first + threadIdx.x, n - 1), l1 = min(first + threadIdx.x + kProjBlock, n - 1);
+    // a thread whose second splat is beyond the array takes its first one twice, one with neither leaves its slots as they are (what
+    // it then computes is not stored); clamping to the last splat made the blocks of a split over views queue for one address
+    const int64_t l0 = first + threadIdx.x, l1 = l0 + kProjBlock < n ? l0 + kProjBlock : l0;
+    if (l0 < n) {
         if (ROWS && n_sh > 0) {
             const uint32_t s = (uint32_t)__cvta_generic_to_shared(&in.row[0][threadIdx.x]);
 #pragma unroll
@@ -571,6 +582,7 @@ __device__ __forceinline__ void to_azimuthal(Pair A[16 * 3], const Pair W[kShPer
 // What the registers allow (150 and 252 per thread); the grids are this many blocks, which walk the tiles.  Four forward blocks
 // make the compiler spill: 73 us against 64.
 constexpr int kFwdBlocksPerSm = 3, kBwdBlocksPerSm = 2;
+constexpr int kMaxSplit = 8;                   // blocks that share a tile's views in the backward pass, a cluster
 
 // Per (splat, view): the direction (12 operations), the azimuthal functions (7) and 45 multiply-adds.  1M splats, 16 views: 64 us;
 // 20.8M packed instructions at the three cycles of the register file are 55 us, the bytes (248 MB) 38 us.
@@ -583,7 +595,9 @@ __global__ void __launch_bounds__(kProjBlock, kFwdBlocksPerSm) sh_eval_fwd_views
     __shared__ TileInputs in;
     float* sh_s = (float*)dyn_s;
     const bool with_dc = sp.features_dc != nullptr;
-    const int64_t stride = (int64_t)gridDim.x * kEvalTile;
+    const int64_t stride = (int64_t)gridDim.x * kEvalTile, from = share_of_views(views);
+    viewmats += 16 * from;
+    out += 3 * from * n;
     fetch_inputs<ROWS>(in, sp, with_dc, shq.packed, n_sh, (int64_t)blockIdx.x * kEvalTile, n);
     stage_centres(centres_s, viewmats, 0, views);
     __syncthreads();
@@ -667,6 +681,27 @@ __device__ __forceinline__ void fetch_grads(GradRing& ring, int slot, GradCursor
     asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
+// dst[k] = the sum over the cluster's blocks of their span[k], for this block's share of k; spans are 16-byte aligned.  The loads of
+// a step are independent: one float at a time the join of 24 tiles took 12 us.
+__device__ __forceinline__ void join_span(float* dst, float* span_s, int count, bool add) {
+    const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+    const int blocks = (int)gridDim.y, quads = (count + 3) / 4, from = quads * (int)blockIdx.y / blocks, to = quads * ((int)blockIdx.y + 1) / blocks;
+#pragma unroll 4
+    for (int k = from + threadIdx.x; k < to; k += kProjBlock) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int q = 0; q < kMaxSplit; ++q)
+            if (q < blocks) {
+                const float4 b = *(const float4*)cluster.map_shared_rank(span_s + 4 * k, q);
+                a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+            }
+        const float e[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (4 * k + j < count) dst[4 * k + j] = add ? dst[4 * k + j] + e[j] : e[j];
+    }
+}
+
 // Per (splat, view): direction and polynomials (35 operations), 45 multiply-adds for the coefficients' gradients, 45 for the sums w_j
 // and 40 for the mean's.  The 45 gradients of both splats stay in registers over all views, so nothing is added in memory and the sum
 // has one order.  1M splats, 16 views: 154 us; 47.5M packed instructions at three cycles are 125 us, the bytes (440 MB) 67 us.
@@ -681,7 +716,9 @@ __global__ void __launch_bounds__(kProjBlock, kBwdBlocksPerSm) sh_eval_bwd_views
     __shared__ TileInputs in;
     __shared__ ViewCentre<Pair> centres_s[kCentreChunk];
     float* sh_s = (float*)dyn_s;                 // values on the way in, their gradients on the way out
-    const int64_t stride = (int64_t)gridDim.x * kEvalTile;
+    const int64_t stride = (int64_t)gridDim.x * kEvalTile, from = share_of_views(views);
+    viewmats += 16 * from;
+    v_out += 3 * from * n;
     GradCursor ahead;
     int slot = 0;
     cursor_tile(ahead, v_out, n, (int64_t)blockIdx.x * kEvalTile);
@@ -689,7 +726,7 @@ __global__ void __launch_bounds__(kProjBlock, kBwdBlocksPerSm) sh_eval_bwd_views
     for (int k = 0; k < kGradAhead && views > 0; ++k) fetch_grads(ring, k, ahead, v_out, n, views, stride);
     stage_centres(centres_s, viewmats, 0, views);
     for (int64_t first = (int64_t)blockIdx.x * kEvalTile; first < n; first += stride) {
-        const int64_t i0 = first + threadIdx.x, i1 = i0 + kProjBlock, l0 = min(i0, n - 1), l1 = min(i1, n - 1);
+        const int64_t i0 = first + threadIdx.x, i1 = i0 + kProjBlock;
         __syncthreads();
         if (!ROWS) stage_tile(sh_s, dyn_s + kEvalShBytes, sp, shq, first, n);
         // at least `views` groups were begun after the tile's inputs, the last kGradAhead of which may be under way
@@ -736,12 +773,11 @@ __global__ void __launch_bounds__(kProjBlock, kBwdBlocksPerSm) sh_eval_bwd_views
             }
         }
         float e0[6 + kShPerSplat], e1[6 + kShPerSplat];
-        const bool checked = !(least > kSquareMin && most < kSquareMax);
+        const bool checked = !(least > kSquareMin && most < kSquareMax) && i0 < n;
         if (checked) {
             const void* rows = ROWS && n_sh > 0 ? shq.packed : nullptr;
-            eval_checked(sp, sh_s + threadIdx.x * kShPerSplat, rows, l0, n, views, viewmats, n_sh, nullptr, v_out, e0);
-            // the second splat's values exist only inside the array
-            if (i1 < n) eval_checked(sp, sh_s + (threadIdx.x + kProjBlock) * kShPerSplat, rows, l1, n, views, viewmats, n_sh, nullptr, v_out, e1);
+            eval_checked(sp, sh_s + threadIdx.x * kShPerSplat, rows, i0, n, views, viewmats, n_sh, nullptr, v_out, e0);
+            if (i1 < n) eval_checked(sp, sh_s + (threadIdx.x + kProjBlock) * kShPerSplat, rows, i1, n, views, viewmats, n_sh, nullptr, v_out, e1);
         }
         bulk_done();
         __syncthreads();          // the previous tile's copies have left, and every thread has read its values
@@ -762,9 +798,17 @@ __global__ void __launch_bounds__(kProjBlock, kBwdBlocksPerSm) sh_eval_bwd_views
             for (int k = 0; k < 3; ++k) { mean_s[3 * t0 + k] = e0[k]; mean_s[3 * t1 + k] = e1[k]; dc_s[3 * t0 + k] = e0[3 + k]; dc_s[3 * t1 + k] = e1[3 + k]; }
             for (int k = 0; k < kShPerSplat; ++k) { sh_s[kShPerSplat * t0 + k] = e0[6 + k]; sh_s[kShPerSplat * t1 + k] = e1[6 + k]; }
         }
+        const int count = (int)min((int64_t)kEvalTile, n - first);
+        if (gridDim.y > 1) {      // the tile's blocks form a cluster: each adds up its part of the spans over all of them, in view order
+            cooperative_groups::this_cluster().sync();
+            if (gr.means) join_span(gr.means + 3 * first, mean_s, 3 * count, accumulate != 0);
+            if (gr.features_dc) join_span(gr.features_dc + 3 * first, dc_s, 3 * count, accumulate != 0);
+            if (gr.features_sh) join_span(gr.features_sh + kShPerSplat * first, sh_s, kShPerSplat * count, accumulate != 0);
+            cooperative_groups::this_cluster().sync();      // nobody leaves, or writes its spans again, while they are being read
+            continue;
+        }
         span_written();
         __syncthreads();
-        const int count = (int)min((int64_t)kEvalTile, n - first);
         if (gr.means) store_span(gr.means + 3 * first, mean_s, 3 * count, 3 * kEvalTile, accumulate != 0);
         if (gr.features_dc) store_span(gr.features_dc + 3 * first, dc_s, 3 * count, 3 * kEvalTile, accumulate != 0);
         if (gr.features_sh) store_span(gr.features_sh + kShPerSplat * first, sh_s, kShPerSplat * count, kShPerSplat * kEvalTile, accumulate != 0);
@@ -808,7 +852,9 @@ int ssb_sh_eval_fwd(const SsbSplats* splats, const SsbShQuant* shq, int64_t n, c
     } else if (cams->count == 1) {
         sh_eval_fwd_staged_kernel<<<tiles, kRowBlock, 0, st>>>(*splats, q, n, cams->d_viewmats, n_sh, d_values);
     } else {
-        const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(n, kEvalTile), 148 * kFwdBlocksPerSm);
+        const unsigned resident = 148 * kFwdBlocksPerSm, tiles2 = (unsigned)std::min<int64_t>(ceil_div(n, kEvalTile), resident);
+        // few tiles: their views over the blocks that fit beside them (1 splat and 1 000 views 157 -> 3.9 us, 6 007 and 16 5.2 -> 4.1)
+        const dim3 blocks(tiles2, std::max(1u, std::min((unsigned)cams->count, resident / tiles2)));
         constexpr int smem = kEvalShBytes + kShRawBytes;
         if (rows) sh_eval_fwd_views_kernel<true><<<blocks, kProjBlock, 0, st>>>(*splats, q, n, cams->count, cams->d_viewmats, n_sh, d_values);
         else {
@@ -838,12 +884,21 @@ int ssb_sh_eval_bwd(const SsbSplats* splats, const SsbShQuant* shq, int64_t n, c
         if (rows) sh_eval_bwd_one_kernel<true><<<tiles, kRowBlock, 0, st>>>(*splats, q, n, cams->d_viewmats, n_sh, d_v_values, *grads, accumulate);
         else sh_eval_bwd_one_kernel<false><<<tiles, kRowBlock, 0, st>>>(*splats, q, n, cams->d_viewmats, n_sh, d_v_values, *grads, accumulate);
     } else {
-        const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(n, kEvalTile), 148 * kBwdBlocksPerSm);
-        const void* kernel = rows ? (const void*)sh_eval_bwd_views_kernel<true> : (const void*)sh_eval_bwd_views_kernel<false>;
+        const unsigned resident = 148 * kBwdBlocksPerSm, tiles = (unsigned)std::min<int64_t>(ceil_div(n, kEvalTile), resident);
+        // Few tiles and many views: a tile's views over a cluster of blocks.  A view costs a tile about 0.4 us, the join 3.5: 300 splats
+        // and 70 views 37 -> 10 us, 6 007 and 16 10.8 -> 8.8, but 6 007 and 4 6.0 -> 8.5.
+        unsigned split = 1;
+        while (cams->count >= 16 && split < kMaxSplit && 2 * split * tiles <= resident && 2 * (int64_t)split <= cams->count / 2) split *= 2;
+        auto* kernel = rows ? sh_eval_bwd_views_kernel<true> : sh_eval_bwd_views_kernel<false>;
         const int smem = kEvalShBytes + (rows ? 0 : kShRawBytes);
-        if (int e = ensure_dynamic_smem(kernel, smem)) return e;
-        if (rows) sh_eval_bwd_views_kernel<true><<<blocks, kProjBlock, smem, st>>>(*splats, q, n, cams->count, cams->d_viewmats, n_sh, d_v_values, *grads, accumulate);
-        else sh_eval_bwd_views_kernel<false><<<blocks, kProjBlock, smem, st>>>(*splats, q, n, cams->count, cams->d_viewmats, n_sh, d_v_values, *grads, accumulate);
+        if (int e = ensure_dynamic_smem((const void*)kernel, smem)) return e;
+        cudaLaunchAttribute cluster;
+        cluster.id = cudaLaunchAttributeClusterDimension;
+        cluster.val.clusterDim.x = 1; cluster.val.clusterDim.y = split; cluster.val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(tiles, split); cfg.blockDim = dim3(kProjBlock); cfg.dynamicSmemBytes = (size_t)smem; cfg.stream = st;
+        cfg.attrs = &cluster; cfg.numAttrs = split > 1 ? 1 : 0;
+        SSB_CUDA(cudaLaunchKernelEx(&cfg, kernel, *splats, q, n, (int)cams->count, cams->d_viewmats, n_sh, d_v_values, *grads, accumulate));
     }
     SSB_LAUNCHED("sh_eval_bwd_kernel");
     return SSB_OK;

@@ -355,7 +355,10 @@ def run_bwd(lib, c, src, degree=3, accumulate=0, base=None, want=("means", "feat
 
 @pytest.mark.parametrize("fmt", [4, 8, 16, 32])
 @pytest.mark.parametrize("n,views,degree,shift", [(1, 1, 3, 0), (5, 2, 2, 1), (127, 1, 3, 2), (128, 3, 3, 0), (129, 1, 1, 3), (1000, 16, 3, 1),
-                                                  (1000, 1, 0, 0), (4001, 33, 3, 0), (300, 70, 2, 0), (20003, 1, 3, 1), (20004, 1, 3, 0)])
+                                                  (1000, 1, 0, 0), (4001, 33, 3, 0), (300, 70, 2, 0), (20003, 1, 3, 1), (20004, 1, 3, 0),
+                                                  # few splats and many views: the views split over blocks, at the edges of the split
+                                                  (1, 1000, 3, 0), (257, 4, 3, 0), (6007, 16, 3, 1), (9472, 9, 3, 0), (18945, 15, 1, 0), (37888, 4, 3, 0), (37889, 4, 3, 0),
+                                                  (64, 3, 3, 2)])
 def test_eval_forward_and_backward(lib, fmt, n, views, degree, shift):
     c = eval_case(n, views)
     src = sources(lib, c["sh"], fmt)
