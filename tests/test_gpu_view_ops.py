@@ -571,17 +571,17 @@ def test_eval_of_more_than_2_31_outputs_and_gradients(lib):
     within(gm[-k:], wm, tm); within(gs[-k:].reshape(k, 15, 3), ws, ts)
 
 
-def test_calls_on_several_streams_at_once_and_repeated_calls_agree(lib):
-    c = eval_case(60_000, 5)
+@pytest.mark.parametrize("n,views", [(60_000, 5), (3000, 20)])       # whole tiles per block; views split over a cluster
+def test_calls_on_several_streams_at_once_and_repeated_calls_agree(lib, n, views):
+    c = eval_case(n, views)
     src = sources(lib, c["sh"], 4)
     m, dc, vm, v, sh = dev(c["means"]), dev(c["dc"]), dev(c["vm"]), dev(c["v"]), dev(c["sh"])
     sp = L.splats_struct(dict(means=m, features_dc=dc))
     cams = L.cameras_struct(vm, vm, 1, 1)
     d = L.dropout_struct(0.3, 1, 2)
-    n = 60_000
 
     def work(stream):
-        out, gm, gs = torch.empty(5, n, 3, device=DEV), torch.empty(n, 3, device=DEV), torch.empty(n, 45, device=DEV)
+        out, gm, gs = torch.empty(views, n, 3, device=DEV), torch.empty(n, 3, device=DEV), torch.empty(n, 45, device=DEV)
         y, rows = torch.empty(n * 45, device=DEV), torch.empty(n, 32, dtype=torch.uint8, device=DEV)
         g = L.splats_struct(dict(means=gm, features_sh=gs))
         torch.cuda.synchronize()

@@ -291,14 +291,14 @@ def test_first_calls_inside_a_capture():
 import ctypes as C, torch
 from spirula_studio_b200 import lib as L
 lib = L.load()
-n, V = 500, 3
+n, V = 500, 20
 x = torch.randn(n * 45, device="cuda"); y = torch.zeros_like(x); rows = torch.zeros(n, 32, dtype=torch.uint8, device="cuda")
 m = torch.randn(n, 3, device="cuda"); vm = torch.eye(4, device="cuda").reshape(1, 16).repeat(V, 1).contiguous()
 out = torch.zeros(V, n, 3, device="cuda"); g = torch.zeros(n, 45, device="cuda"); gm = torch.zeros(n, 3, device="cuda")
 d = L.dropout_struct(0.3, 1, 2)
 sp = L.splats_struct(dict(means=m)); spf = L.splats_struct(dict(means=m, features_sh=y)); gr = L.splats_struct(dict(means=gm, features_sh=g))
 q = L.shq_struct(rows, None, 4, 0)
-cams = L.cameras_struct(vm, vm, 1, 1); one = L.cameras_struct(vm, vm, 1, 1, count=1)
+cams = L.cameras_struct(vm, vm, 1, 1); one, three = (L.cameras_struct(vm, vm, 1, 1, count=k) for k in (1, 3))
 torch.cuda.synchronize()
 graph = torch.cuda.CUDAGraph()
 with torch.cuda.graph(graph):
@@ -310,7 +310,7 @@ with torch.cuda.graph(graph):
     L.check(lib.ssb_quant_encode(L.ptr(y), n * 45, 4, L.ptr(rows), None, st))
     L.check(lib.ssb_quant_decode(L.ptr(rows), None, n * 45, 4, L.ptr(g), st))
     for s, shq in ((sp, C.byref(q)), (spf, None)):
-        for c in (one, cams):
+        for c in (one, three, cams):
             L.check(lib.ssb_sh_eval_fwd(C.byref(s), shq, n, C.byref(c), L.ptr(out), st))
             L.check(lib.ssb_sh_eval_bwd(C.byref(s), shq, n, C.byref(c), L.ptr(out), C.byref(gr), 0, st))
 graph.replay()
