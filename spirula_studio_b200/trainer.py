@@ -78,8 +78,8 @@ class DropoutOptions:
     """Dropout for captures with few views (ssb_dropout_opacities, ssb_dropout): every iteration each splat is left out of all
     views with probability splat_rate, the other opacities compensated; and each group of sh_group consecutive SH values (1 a value,
     3 a coefficient's three colours, 45 a splat's row) is left out with probability sh_rate.  The masks are functions of the seed and
-    the iteration number, the same on every rank.  Rates can change from iteration to iteration (Trainer.set_dropout).  render()
-    never drops anything."""
+    the iteration number, the same on every rank.  Rates can change from iteration to iteration (Trainer.set_dropout).  The gradients
+    that a call of the trainer leaves in `grads` are those of the stored parameters.  render() never drops anything."""
     splat_rate: float = 0.0
     sh_rate: float = 0.0
     sh_group: int = 3
@@ -213,9 +213,8 @@ class Trainer:
         self.view_sh_bits = view_sh_bits
         self.dropout = None
         self._view_opacities = self._view_sh = self._sh_rows = self._render_rows = None
-        self._dropped = None                 # this iteration's (splat, SH) descriptions between its views and its optimiser step
+        self._view_grads = {}                # gradients of the dropped arrays, where views accumulate into `grads`
         self._v_struct, self._v_shq = self._p_struct, self.shq
-        self._views_open = False
         if dropout is not None:
             self.dropout = DropoutOptions(sh_group=dropout.sh_group, seed=dropout.seed)
             self.set_dropout(dropout.splat_rate, dropout.sh_rate)
@@ -387,7 +386,8 @@ class Trainer:
         own = sum(t.numel() * t.element_size() for t in (self.params_flat, self.grads_flat, self.m1_flat, self.m2_flat))
         if self.quant:
             own += sum(t.numel() * t.element_size() for t in (self.sh_packed, self.sh_bounds, self.sh_optim_packed, self.sh_optim_bounds))
-        own += sum(t.numel() * t.element_size() for t in (self._view_opacities, self._view_sh, self._sh_rows, self._render_rows) if t is not None)
+        own += sum(t.numel() * t.element_size() for t in (self._view_opacities, self._view_sh, self._sh_rows, self._render_rows, *self._view_grads.values())
+                   if t is not None)
         return own + sum(int(self.lib.ssb_step_device_bytes(h)) for h in self.handles)
 
     # -- pieces ------------------------------------------------------------
@@ -405,7 +405,7 @@ class Trainer:
 
     # -- what the views read -----------------------------------------------
     def set_dropout(self, splat_rate=0.0, sh_rate=0.0):
-        """Dropout rates of the following iterations, each in [0, 1)."""
+        """Dropout rates of the following calls that run views, each in [0, 1)."""
         for rate in (splat_rate, sh_rate):
             if not 0.0 <= rate < 1.0:
                 raise ValueError(f"dropout rates must be in [0, 1), not {rate}")
@@ -426,10 +426,14 @@ class Trainer:
         L.check(self.lib.ssb_quant_encode(L.ptr(values), self.n * 45, 4, L.ptr(rows), None, stream))
         return rows, L.shq_struct(rows, None, 4, 0)
 
-    def _begin_views(self, stream=None):
-        """Before an iteration's first view: makes the arrays its views read."""
+    def _on(self, stream):
+        """Torch's current stream set to the one that a call was given (a raw handle; None: the legacy default stream)."""
+        raw = getattr(stream, "value", stream)
+        return torch.cuda.stream(torch.cuda.ExternalStream(raw, device=self.device) if raw else torch.cuda.default_stream(self.device))
+
+    def _begin_views(self, stream):
+        """Makes the arrays that the views of a call read; returns the call's dropout, (splat, SH, group) with None for what is off."""
         d, i = self.dropout, self.iteration
-        self._views_open, self._dropped, self._dropped_stream = True, None, stream
         views, shq = dict(self.params), self.shq
         if self.quant:
             views["features_sh"] = None
@@ -447,26 +451,55 @@ class Trainer:
             views["features_sh"] = self._view_sh
         if self.view_sh_bits == 4:
             self._sh_rows, shq = self._encode_rows(views["features_sh"], self._sh_rows, stream)
-        if splat is not None or sh is not None:
-            self._dropped = (splat, sh, d.sh_group)
-            self._v_struct = L.splats_struct(views)
-        else:
-            self._v_struct = self._p_struct
+        self._v_struct = L.splats_struct(views) if splat is not None or sh is not None else self._p_struct
         self._v_shq = shq
+        return splat, sh, d.sh_group if d is not None else 1
 
-    def _end_views(self):
-        """After an iteration's last view: gradients of what the views read become gradients of the stored parameters."""
-        self._views_open = False
-        if self._dropped is None:
-            return
-        (splat, sh, group), stream = self._dropped, self._dropped_stream
-        self._dropped = None
+    def _end_views(self, dropped, grads, stream):
+        """Gradients of what a call's views read, in `grads`, become gradients of the stored parameters in place."""
+        splat, sh, group = dropped
         if splat is not None:
-            g = self.grads["opacities"]
+            g = grads["opacities"]
             L.check(self.lib.ssb_dropout_opacities_bwd(L.ptr(self.params["opacities"]), L.ptr(g), 0, self.n, C.byref(splat), L.ptr(g), stream))
         if sh is not None:
-            g = self.grads["features_sh"]
+            g = grads["features_sh"]
             L.check(self.lib.ssb_dropout(L.ptr(g), 0, self.n * 45, group, C.byref(sh), L.ptr(g), stream))
+
+    def _run_views(self, batches, accumulate=False, stream=None):
+        """Forward + loss + backward of the views of `batches` = [(kind, d_viewmats, d_intrins, d_gt, n_views, events or None)], one event
+        handle per view that its target waits for.  When it returns, everything up to the gradients of the stored parameters is
+        enqueued on `stream`: what the views left in `grads`, or added to it, is not touched by a later call."""
+        dropped = self._begin_views(stream)
+        # Dropped arrays' gradients take the chain rule in place; where they are to be added to what `grads` holds, which is the
+        # stored parameters' already, the views write them to arrays of their own first.
+        own = {}
+        if accumulate:
+            for name, d in (("opacities", dropped[0]), ("features_sh", dropped[1])):
+                if d is not None:
+                    if name not in self._view_grads:
+                        self._view_grads[name] = torch.empty_like(self.grads[name])
+                    own[name] = self._view_grads[name]
+        if own:
+            with self._on(stream):
+                for g in own.values():
+                    g.zero_()
+        grads = {**self.grads, **own}
+        g_struct = L.splats_struct(grads) if own else self._g_struct
+        for i, (kind, d_viewmats, d_intrins, d_gt, n_views, events) in enumerate(batches):
+            add = accumulate or i > 0
+            if self.fused_backward:
+                self._keep_cams(d_viewmats, d_intrins, n_views, not add)
+            # one call per camera kind: each view's loss stage waits on the device for its own target
+            L.check(self.lib.ssb_step_views_gated(self.handles[kind], C.byref(self._v_struct), C.byref(self._v_shq) if self._v_shq else None,
+                                                  L.ptr(d_viewmats), L.ptr(d_intrins), L.ptr(d_gt), n_views, events,
+                                                  C.byref(g_struct), 1 if add else 0, L.ptr(self.losses), stream))
+        if not any(b[4] > 0 for b in batches):
+            return                           # no view: `grads` is as it was
+        self._end_views(dropped, grads, stream)
+        if own:
+            with self._on(stream):
+                for name, g in own.items():
+                    self.grads[name].add_(g)
 
     def render(self, viewmat, intrin, kind=0, depth=False, sh_bits=None):
         """One image of the current splats, forward only (the viewer's path): viewmat [16] / intrin [4] as numpy or tensors.
@@ -518,19 +551,13 @@ class Trainer:
         L.check(self.lib.ssb_step_set_distortion(self.handles[kind], int(tier), L.ptr(rows) if rows is not None else None))
 
     def views_fwd_bwd(self, d_viewmats, d_intrins, d_gt, n_views, accumulate=False, stream=None, kind=0):
-        """Forward + loss + backward of n_views views (all of camera kind `kind`) already resident on the device."""
-        if self.fused_backward:
-            self._keep_cams(d_viewmats, d_intrins, n_views, not accumulate)
-        if not accumulate or not self._views_open:
-            self._begin_views(stream)
-        L.check(self.lib.ssb_step_views(self.handles[kind], C.byref(self._v_struct), C.byref(self._v_shq) if self._v_shq else None,
-                                        L.ptr(d_viewmats), L.ptr(d_intrins), L.ptr(d_gt), n_views,
-                                        C.byref(self._g_struct), 1 if accumulate else 0, L.ptr(self.losses), stream))
+        """Forward + loss + backward of n_views views (all of camera kind `kind`) already resident on the device.  Their gradients, of the
+        stored parameters, replace what `grads` holds or, with accumulate, are added to it, in the order of `stream`."""
+        self._run_views([(kind, d_viewmats, d_intrins, d_gt, n_views, None)], accumulate, stream)
 
     def allreduce_grads(self):
         """Makes the summed gradients available where the optimiser will read them: everywhere ("nccl"),
         or, for this rank's range of splats, in this rank's buffer ("peer")."""
-        self._end_views()
         if self.grad_sync == "nccl":
             torch.distributed.all_reduce(self.grads_flat, op=torch.distributed.ReduceOp.SUM, group=self.pg)
         elif self.grad_sync in ("peer", "multimem"):
@@ -554,7 +581,6 @@ class Trainer:
 
     def optimizer_step(self, total_views, stream=None):
         lr = self.cfg.lrs
-        self._end_views()
         self.iteration += 1
         cfg = L.SsbAdamConfig(lr["lr_means"], lr["lr_quats"], lr["lr_scales"], lr["lr_opacities"], lr["lr_features_dc"],
                               lr["lr_features_sh"], self.optim.sh_reg if self.optim is not None else 0.0, 1.0 / float(total_views), self.iteration, 0)
@@ -635,12 +661,10 @@ class Trainer:
         self.losses.zero_()
         if self.radii is not None and not self._radii_external:
             self.radii.zero_()
-        first = True
-        for kind, d_viewmats, d_intrins, d_gt, nv in batches:
-            if nv > 0:
-                self.views_fwd_bwd(d_viewmats, d_intrins, d_gt, nv, accumulate=not first, kind=kind)
-                first = False
-        if first:
+        batches = [(*b, None) for b in batches if b[4] > 0]
+        if batches:
+            self._run_views(batches)
+        else:
             self.grads_flat.zero_()
         self.allreduce_grads()
         self.optimizer_step(total_views)
@@ -718,20 +742,9 @@ class Trainer:
         if nv_total == 0:
             self.grads_flat.zero_()
         main.wait_event(cams_ready)
-        first = True
-        for kind, nv, handles, keep in calls:
-            if nv == 0:
-                continue
-            d_view, d_intr, d_gt = self._staging[(kind, k)]
-            if self.fused_backward:
-                self._keep_cams(d_view, d_intr, nv, first)
-            if first:
-                self._begin_views()
-            # one call per camera kind: each view's loss stage waits on the device for its own target
-            L.check(self.lib.ssb_step_views_gated(self.handles[kind], C.byref(self._v_struct), C.byref(self._v_shq) if self._v_shq else None,
-                                                  L.ptr(d_view), L.ptr(d_intr), L.ptr(d_gt), nv, handles,
-                                                  C.byref(self._g_struct), 0 if first else 1, L.ptr(self.losses), None))
-            first = False
+        batches = [(kind, *self._staging[(kind, k)], nv, handles) for kind, nv, handles, keep in calls if nv > 0]
+        if batches:
+            self._run_views(batches)
         self._keep_events = [c[3] for c in calls]      # the events must outlive the work that waits on them
         self.allreduce_grads()
         self.optimizer_step(total_views)

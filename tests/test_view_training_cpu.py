@@ -1,0 +1,185 @@
+"""What a Trainer asks of the library around an iteration's views, without a GPU: a stand-in for the library that works on host memory
+and notes every call with its stream.  Its views' gradients are functions of the arrays that the views are given, its dropout calls are
+the oracle's."""
+import contextlib
+import ctypes as C
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import view_ops_oracle as O  # noqa: E402
+from spirula_studio_b200 import lib as L, scenes, trainer as T  # noqa: E402
+from spirula_studio_b200.trainer import DropoutOptions, Trainer  # noqa: E402
+
+N = 37
+
+
+def floats(address, count):
+    address = getattr(address, "value", address)
+    return np.ctypeslib.as_array((C.c_float * count).from_address(address))
+
+
+def handle(stream):
+    return getattr(stream, "value", stream) or 0
+
+
+class StandIn:
+    """Entry points without a method of their own succeed and do nothing."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            own = getattr(self, "_" + name, None) if not name.startswith("_") else None
+            if own is not None:
+                own(*args)
+            self.calls.append((name, args))
+            return 0
+        if name.startswith("_"):
+            raise AttributeError(name)
+        return call
+
+    def names(self):
+        return [n for n, _ in self.calls]
+
+    def _ssb_step_views(self, step, params, shq, vm, K, gt, views, grads, accumulate, losses, stream):
+        self._ssb_step_views_gated(step, params, shq, vm, K, gt, views, None, grads, accumulate, losses, stream)
+
+    def _ssb_step_views_gated(self, step, params, shq, vm, K, gt, views, ready, grads, accumulate, losses, stream):
+        if views == 0:
+            return
+        p, g = params._obj, grads._obj
+        for k, w in (("means", 3), ("quats", 4), ("scales", 3), ("opacities", 1), ("features_dc", 3), ("features_sh", 45)):
+            out = floats(getattr(g, k), N * w)
+            value = views * view_gradient(k, floats(getattr(p, k), N * w))
+            out[:] = out + value if accumulate else value
+
+    def _ssb_dropout(self, x, first, count, group, d, y, stream):
+        d = d._obj
+        floats(y, count)[:] = O.dropout(floats(x, count).copy(), first, group, d.rate, d.seed, d.offset)
+
+    def _ssb_dropout_opacities(self, x, first, count, d, y, stream):
+        d = d._obj
+        floats(y, count)[:] = O.dropout_opacities(floats(x, count).copy(), first, d.rate, d.seed, d.offset)[0]
+
+    def _ssb_dropout_opacities_bwd(self, x, v, first, count, d, out, stream):
+        d = d._obj
+        floats(out, count)[:] = O.dropout_opacities(floats(x, count).copy(), first, d.rate, d.seed, d.offset)[1] * floats(v, count)
+
+
+def view_gradient(name, read):
+    """One view's gradient of the array that it reads."""
+    return (0.5 * read + 1.0) if name in ("opacities", "features_sh") else np.full_like(read, 2.0)
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    lib = StandIn()
+    monkeypatch.setattr(L, "load", lambda: lib)
+    monkeypatch.setattr(Trainer, "_on", lambda self, stream: contextlib.nullcontext(), raising=False)
+    return lib
+
+
+def make(fake, kinds=1, **kw):
+    cfg = scenes.scaled(scenes.CONFIGS["plumbing_50k" if kinds == 1 else "wide_5m"], n_splats=N, width=64, height=48, n_views=2)
+    tr = Trainer(cfg, scenes.make_splats(cfg), device="cpu", **kw)
+    assert len(tr.handles) == kinds
+    fake.calls.clear()
+    return tr
+
+
+def views(tr, count=2, **kw):
+    tr.views_fwd_bwd(torch.zeros(count, 16), torch.zeros(count, 4), torch.zeros(count, 1), count, **kw)
+
+
+OPTS = DropoutOptions(splat_rate=0.3, sh_rate=0.4, sh_group=3, seed=21)
+
+
+def stored_gradients(tr, count, opts=OPTS):
+    """The chain rule through both dropouts, in 64 bits."""
+    i, p = tr.iteration, {k: v.numpy().copy() for k, v in tr.params.items()}
+    want = {k: count * view_gradient(k, v).astype(np.float64) for k, v in p.items()}
+    if opts.splat_rate:
+        y, slope, _ = O.dropout_opacities(p["opacities"], 0, opts.splat_rate, 2 * opts.seed, i)
+        want["opacities"] = slope * (count * view_gradient("opacities", y))
+    if opts.sh_rate:
+        mask = O.dropout(np.ones(N * 45, np.float32), 0, opts.sh_group, opts.sh_rate, 2 * opts.seed + 1, i)
+        want["features_sh"] = mask * (count * view_gradient("features_sh", mask * p["features_sh"]))
+    return want
+
+
+def same(got, want):
+    """A handful of roundings: the copy the views read, the view's own two, the mask's, the slope's, a sum."""
+    for k in want:
+        assert np.allclose(got[k].numpy(), want[k], rtol=16 * O.U, atol=16 * O.U * np.abs(want[k]).max()), k
+
+
+def test_conversion_runs_in_the_views_call_on_its_stream(fake):
+    """A caller who orders two streams by an event between the calls must find the gradients complete at that event."""
+    tr = make(fake, dropout=OPTS, view_sh_bits=4)
+    want = stored_gradients(tr, 2)
+    views(tr, stream=0x10)
+    launched = [n for n in fake.names() if "dropout" in n]
+    assert sorted(launched) == ["ssb_dropout", "ssb_dropout", "ssb_dropout_opacities", "ssb_dropout_opacities_bwd"]
+    assert all(handle(a[-1]) == 0x10 for n, a in fake.calls)
+    same(tr.grads, want)
+    fake.calls.clear()
+    tr.allreduce_grads()
+    tr.optimizer_step(2, stream=0x20)
+    assert not [n for n in fake.names() if "dropout" in n] and all(handle(a[-1]) == 0x20 for n, a in fake.calls)
+    same(tr.grads, want)
+
+
+@pytest.mark.parametrize("opts", [OPTS, DropoutOptions(splat_rate=0.5, seed=3), DropoutOptions(sh_rate=0.5, sh_group=45, seed=4)])
+def test_accumulation_leaves_the_other_terms_alone(fake, opts):
+    tr = make(fake, dropout=opts)
+    want = stored_gradients(tr, 2, opts)
+    for k, g in tr.grads.items():
+        g.copy_(torch.linspace(-3, 3, g.numel()))
+    base = {k: g.numpy().astype(np.float64) for k, g in tr.grads.items()}
+    views(tr, accumulate=True)                                      # into what the caller put there
+    same(tr.grads, {k: base[k] + want[k] for k in want})
+    tr.allreduce_grads()
+    views(tr, accumulate=True)                                      # after the exchange of the first part
+    same(tr.grads, {k: base[k] + 2 * want[k] for k in want})
+    for g in tr.grads.values():
+        g += 1.0                                                    # a regulariser of the caller's
+    tr.optimizer_step(2)
+    same(tr.grads, {k: base[k] + 2 * want[k] + 1.0 for k in want})
+    again = stored_gradients(tr, 2, opts)                           # the next iteration draws its own masks
+    views(tr)
+    same(tr.grads, again)
+
+
+def test_accumulating_views_read_the_parameters_as_they_are(fake):
+    tr = make(fake, dropout=OPTS)
+    first = stored_gradients(tr, 2)
+    views(tr)
+    tr.params["features_sh"].mul_(-2.0)
+    tr.params["opacities"].add_(0.25)
+    second = stored_gradients(tr, 2)
+    views(tr, accumulate=True)
+    same(tr.grads, {k: first[k] + second[k] for k in first})
+
+
+def test_camera_kinds_of_an_iteration_share_one_copy_and_one_conversion(fake):
+    tr = make(fake, kinds=2, dropout=OPTS)
+    want = stored_gradients(tr, 5)
+    batch = lambda kind, n: (kind, torch.zeros(n, 16), torch.zeros(n, 4), torch.zeros(n, 1), n)
+    tr.step_device_kinds([batch(0, 2), batch(1, 0), batch(1, 3)], 5)
+    assert fake.names().count("ssb_dropout") == 2 and fake.names().count("ssb_dropout_opacities_bwd") == 1
+    same(tr.grads, want)
+    tr.step_device_kinds([], 5)
+    assert not any(g.any() for g in tr.grads.values())
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_a_call_without_views_leaves_the_gradients(fake, accumulate):
+    tr = make(fake, dropout=OPTS)
+    want = stored_gradients(tr, 2)
+    views(tr)
+    views(tr, count=0, accumulate=accumulate)
+    same(tr.grads, want)
