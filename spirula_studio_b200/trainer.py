@@ -419,17 +419,24 @@ class Trainer:
             raise ValueError(f"sh_group must be at least 1, not {self.dropout.sh_group}")
         self.dropout.splat_rate, self.dropout.sh_rate = float(splat_rate), float(sh_rate)
 
-    def _encode_rows(self, values, rows, stream=None):
-        """values in 4-bit rows: into `rows`, or a new buffer; returns (rows, their SsbShQuant)."""
-        if rows is None:
-            rows = torch.empty(self.n * L.SH_ROW_BYTES, dtype=torch.uint8, device=self.device)
-        L.check(self.lib.ssb_quant_encode(L.ptr(values), self.n * 45, 4, L.ptr(rows), None, stream))
-        return rows, L.shq_struct(rows, None, 4, 0)
-
     def _on(self, stream):
         """Torch's current stream set to the one that a call was given (a raw handle; None: the legacy default stream)."""
         raw = getattr(stream, "value", stream)
         return torch.cuda.stream(torch.cuda.ExternalStream(raw, device=self.device) if raw else torch.cuda.default_stream(self.device))
+
+    def _like(self, t, stream):
+        """A buffer of t's shape that is first written on `stream`: torch's allocator may hand out memory whose last use, on the stream it
+        is asked on, is still under way."""
+        with self._on(stream):
+            return torch.empty_like(t)
+
+    def _encode_rows(self, values, rows, stream=None):
+        """values in 4-bit rows: into `rows`, or a new buffer; returns (rows, their SsbShQuant)."""
+        if rows is None:
+            with self._on(stream):
+                rows = torch.empty(self.n * L.SH_ROW_BYTES, dtype=torch.uint8, device=self.device)
+        L.check(self.lib.ssb_quant_encode(L.ptr(values), self.n * 45, 4, L.ptr(rows), None, stream))
+        return rows, L.shq_struct(rows, None, 4, 0)
 
     def _begin_views(self, stream):
         """Makes the arrays that the views of a call read; returns the call's dropout, (splat, SH, group) with None for what is off."""
@@ -441,12 +448,12 @@ class Trainer:
         sh = L.dropout_struct(d.sh_rate, (2 * d.seed + 1) & 0xffffffffffffffff, i) if d is not None and d.sh_rate > 0.0 else None
         if splat is not None:
             if self._view_opacities is None:
-                self._view_opacities = torch.empty_like(self.params["opacities"])
+                self._view_opacities = self._like(self.params["opacities"], stream)
             L.check(self.lib.ssb_dropout_opacities(L.ptr(self.params["opacities"]), 0, self.n, C.byref(splat), L.ptr(self._view_opacities), stream))
             views["opacities"] = self._view_opacities
         if sh is not None:
             if self._view_sh is None:
-                self._view_sh = torch.empty_like(self.params["features_sh"])
+                self._view_sh = self._like(self.params["features_sh"], stream)
             L.check(self.lib.ssb_dropout(L.ptr(self.params["features_sh"]), 0, self.n * 45, d.sh_group, C.byref(sh), L.ptr(self._view_sh), stream))
             views["features_sh"] = self._view_sh
         if self.view_sh_bits == 4:
@@ -477,7 +484,7 @@ class Trainer:
             for name, d in (("opacities", dropped[0]), ("features_sh", dropped[1])):
                 if d is not None:
                     if name not in self._view_grads:
-                        self._view_grads[name] = torch.empty_like(self.grads[name])
+                        self._view_grads[name] = self._like(self.grads[name], stream)
                     own[name] = self._view_grads[name]
         if own:
             with self._on(stream):

@@ -183,3 +183,27 @@ def test_a_call_without_views_leaves_the_gradients(fake, accumulate):
     views(tr)
     views(tr, count=0, accumulate=accumulate)
     same(tr.grads, want)
+
+
+def test_buffers_are_allocated_on_the_stream_that_writes_them(fake, monkeypatch):
+    """torch's allocator orders the reuse of memory by the stream it is asked on."""
+    tr = make(fake, dropout=OPTS, view_sh_bits=4)
+    current, asked = [None], []
+
+    @contextlib.contextmanager
+    def on(self, stream):
+        before, current[0] = current[0], handle(stream)
+        yield
+        current[0] = before
+    monkeypatch.setattr(Trainer, "_on", on, raising=False)
+    for name in ("empty", "empty_like"):
+        real = getattr(torch, name)
+        monkeypatch.setattr(torch, name, lambda *a, real=real, **kw: asked.append(current[0]) or real(*a, **kw))
+    views(tr, stream=0x10)
+    assert asked == [0x10] * 3                       # opacities, SH values, rows
+    del asked[:]
+    views(tr, accumulate=True, stream=0x20)
+    assert asked == [0x20] * 2                       # their gradients
+    del asked[:]
+    views(tr, accumulate=True, stream=0x20)
+    assert not asked
