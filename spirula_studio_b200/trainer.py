@@ -212,7 +212,8 @@ class Trainer:
             raise ValueError("view_sh_bits=4 needs fp32 SH values (sh_value_bits = 32)")
         self.view_sh_bits = view_sh_bits
         self.dropout = None
-        self._view_opacities = self._view_sh = self._sh_rows = self._render_rows = None
+        self._view_opacities = self._view_sh = self._sh_rows = None
+        self._render_rows = {}               # camera kind: (rows, event after the last render that reads them)
         self._view_grads = {}                # gradients of the dropped arrays, where views accumulate into `grads`
         self._v_struct, self._v_shq = self._p_struct, self.shq
         if dropout is not None:
@@ -386,8 +387,8 @@ class Trainer:
         own = sum(t.numel() * t.element_size() for t in (self.params_flat, self.grads_flat, self.m1_flat, self.m2_flat))
         if self.quant:
             own += sum(t.numel() * t.element_size() for t in (self.sh_packed, self.sh_bounds, self.sh_optim_packed, self.sh_optim_bounds))
-        own += sum(t.numel() * t.element_size() for t in (self._view_opacities, self._view_sh, self._sh_rows, self._render_rows, *self._view_grads.values())
-                   if t is not None)
+        own += sum(t.numel() * t.element_size() for t in (self._view_opacities, self._view_sh, self._sh_rows, *self._view_grads.values(),
+                                                              *(rows for rows, _ in self._render_rows.values())) if t is not None)
         return own + sum(int(self.lib.ssb_step_device_bytes(h)) for h in self.handles)
 
     # -- pieces ------------------------------------------------------------
@@ -523,12 +524,22 @@ class Trainer:
         rgb = torch.empty(height, width, 3, device=self.device)
         T = torch.empty(height, width, device=self.device)
         dep = torch.empty(height, width, device=self.device) if depth else None
-        stream = C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+        current = torch.cuda.current_stream(self.device)
+        stream = C.c_void_p(current.cuda_stream)
         shq = self.shq
-        if sh_bits == 4:        # a buffer of its own: an iteration's views may be under way on theirs
-            self._render_rows, shq = self._encode_rows(self.params["features_sh"], self._render_rows, stream)
+        if sh_bits == 4:
+            # a buffer of its own (an iteration's views may be under way on theirs) per camera kind, as the step objects are; a render on
+            # another stream may still be reading it
+            rows, done = self._render_rows.get(kind, (None, None))
+            if done is not None:
+                current.wait_event(done)
+            rows, shq = self._encode_rows(self.params["features_sh"], rows, stream)
         L.check(self.lib.ssb_step_render(self.handles[kind], C.byref(self._p_struct), C.byref(shq) if shq else None, L.ptr(d_vm), L.ptr(d_K),
                                          L.ptr(rgb), L.ptr(dep) if depth else None, L.ptr(T), stream))
+        if sh_bits == 4:
+            done = done or torch.cuda.Event()
+            done.record(current)
+            self._render_rows[kind] = (rows, done)
         return (rgb, T, dep) if depth else (rgb, T)
 
     def set_sh_degree(self, degree):

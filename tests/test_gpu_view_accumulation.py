@@ -28,7 +28,7 @@ def scene(n=2500, views=3, w=160, h=112, of="plumbing_50k"):
     cfg.rig = "ring"
     sp = scenes.make_splats(cfg)
     vm, K = scenes.make_cameras(cfg)
-    gt = np.stack([scenes.make_target(cfg, v) for v in range(views)])
+    gt = np.stack([scenes.make_target(cfg, v) for v in range(views)]) if not cfg.view_kinds else None
     return cfg, sp, vm, K, gt
 
 
@@ -101,4 +101,30 @@ def test_accumulation_over_parts_streams_and_foreign_terms():
     torch.cuda.synchronize()
     for k in ref:
         assert close(tr.grads[k], base[k] + ref[k]), k
+    tr.close()
+
+
+def test_renders_from_rows_on_several_streams():
+    """Two camera kinds and two streams taking turns while the values change: each image is that of a trainer with its values."""
+    cfg, sp, vm, K, _ = scene(n=4000, views=2, of="wide_5m")
+    tr = Trainer(cfg, sp, device=DEV)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    start = tr.params["features_sh"].clone()
+    torch.cuda.synchronize()
+    images, last = [], None
+    for i in range(12):
+        s = streams[i // 2 % 2]
+        if last is not None:
+            s.wait_event(last)                           # the change of values waits for the renders of the ones before
+        with torch.cuda.stream(s):
+            tr.params["features_sh"].copy_(start * (1 + i // 4))
+            images.append((i % 2, 1 + i // 4, tr.render(vm[i % 2], K[i % 2], kind=i % 2, sh_bits=4)[0]))
+        last = torch.cuda.Event()
+        last.record(s)
+    torch.cuda.synchronize()
+    assert len(tr._render_rows) == 2
+    for kind, factor, image in images:
+        ref = Trainer(cfg, {**sp, "features_sh": sp["features_sh"] * np.float32(factor)}, device=DEV)
+        assert torch.equal(image, ref.render(vm[kind], K[kind], kind=kind, sh_bits=4)[0])
+        ref.close()
     tr.close()

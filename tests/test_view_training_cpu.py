@@ -207,3 +207,40 @@ def test_buffers_are_allocated_on_the_stream_that_writes_them(fake, monkeypatch)
     del asked[:]
     views(tr, accumulate=True, stream=0x20)
     assert not asked
+
+
+def test_rows_of_renders_on_several_streams(fake, monkeypatch):
+    """A camera kind's renders share a buffer and are ordered by an event; those of another kind have their own."""
+    tr = make(fake, kinds=2)
+    log = fake.calls
+
+    class Stream:
+        def __init__(self, handle):
+            self.cuda_stream = handle
+
+        def wait_event(self, event):
+            log.append(("wait", (event.recorded, self.cuda_stream)))
+
+    class Event:
+        recorded = None
+
+        def record(self, stream):
+            self.recorded = (stream.cuda_stream, len(log))
+            log.append(("record", (stream.cuda_stream,)))
+
+    a, b = Stream(0x10), Stream(0x20)
+    monkeypatch.setattr(torch.cuda, "Event", Event)
+    encoded = []
+    for stream, kind in ((a, 0), (b, 1), (b, 0), (a, 1), (a, 0)):
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None, stream=stream: stream)
+        del log[:]
+        tr.render(np.eye(4), np.ones(4), kind=kind, sh_bits=4)
+        names = fake.names()
+        first = kind not in [k for k, _, _ in encoded]
+        assert names == ([] if first else ["wait"]) + ["ssb_quant_encode", "ssb_step_render", "record"]
+        if not first:
+            last = [s for k, s, _ in encoded if k == kind][-1]
+            assert log[0][1][0][0] == last.cuda_stream
+        assert all(handle(args[-1]) == stream.cuda_stream for _, args in log)
+        encoded.append((kind, stream, handle(dict(log)["ssb_quant_encode"][3])))
+    assert len({p for _, _, p in encoded}) == 2 and len({(k, p) for k, _, p in encoded}) == 2
