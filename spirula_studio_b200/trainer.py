@@ -406,18 +406,18 @@ class Trainer:
 
     # -- what the views read -----------------------------------------------
     def set_dropout(self, splat_rate=0.0, sh_rate=0.0):
-        """Dropout rates of the following calls that run views, each in [0, 1)."""
+        """Dropout rates of the following calls that run views, each in [0, 1) as an fp32 number."""
         for rate in (splat_rate, sh_rate):
-            if not 0.0 <= rate < 1.0:
-                raise ValueError(f"dropout rates must be in [0, 1), not {rate}")
+            if not (0.0 <= rate < 1.0 and np.float32(rate) < 1.0):
+                raise ValueError(f"dropout rates must be in [0, 1) in fp32, not {rate}")
         if (splat_rate > 0.0 or sh_rate > 0.0) and self.fused_backward:
             raise NotImplementedError("dropout runs with the per-view backward (the fused one hands its gradients straight to the optimiser)")
         if sh_rate > 0.0 and self.quant:
             raise ValueError("SH dropout needs fp32 SH values (sh_value_bits = 32)")
         if self.dropout is None:
             self.dropout = DropoutOptions()
-        if self.dropout.sh_group < 1:
-            raise ValueError(f"sh_group must be at least 1, not {self.dropout.sh_group}")
+        if not 1 <= self.dropout.sh_group < 2 ** 31:
+            raise ValueError(f"sh_group must be in [1, 2^31), not {self.dropout.sh_group}")
         self.dropout.splat_rate, self.dropout.sh_rate = float(splat_rate), float(sh_rate)
 
     def _on(self, stream):

@@ -244,3 +244,12 @@ def test_rows_of_renders_on_several_streams(fake, monkeypatch):
         assert all(handle(args[-1]) == stream.cuda_stream for _, args in log)
         encoded.append((kind, stream, handle(dict(log)["ssb_quant_encode"][3])))
     assert len({p for _, _, p in encoded}) == 2 and len({(k, p) for k, _, p in encoded}) == 2
+
+
+@pytest.mark.parametrize("bad", [dict(splat_rate=1.0 - 1e-9), dict(sh_rate=1.0 - 2.0 ** -26), dict(sh_rate=float("nan")), dict(splat_rate=1e300),
+                                 dict(sh_rate=0.1, sh_group=2 ** 31), dict(sh_rate=0.1, sh_group=2 ** 32 + 3), dict(sh_rate=0.1, sh_group=0)])
+def test_options_that_the_library_cannot_take_are_refused_when_they_are_set(fake, bad):
+    """A rate that is one in fp32, a group that 32 bits would cut off: refused here, not in the middle of a run, nor taken for another."""
+    with pytest.raises(ValueError):
+        make(fake, dropout=DropoutOptions(**bad))
+    make(fake, dropout=DropoutOptions(splat_rate=1.0 - 2.0 ** -24, sh_rate=0.0, sh_group=2 ** 31 - 1))
