@@ -214,6 +214,12 @@ __device__ __forceinline__ Directions<T> view_directions(const ViewCentre<T>& c,
     return {dx * inv, dy * inv, dz * inv, inv};
 }
 constexpr float kSquareMin = 1e-30f, kSquareMax = 1e30f;
+// The largest of three, NaN if one is (fmaxf drops them): a square that is not a number left the range too.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 
 template <class T>
 struct Polynomials { T p[kNumSh], ny, x2, t; };        // -y, 2x, z^2 - 1/5
@@ -268,7 +274,7 @@ __device__ __forceinline__ float active_scale(const ShRow& r, int band, int n_sh
 
 // Everything about one splat by the definition, with the direction in double precision, whose range the square of a distance cannot
 // leave: for splats that are nearer to a camera than 1e-15 or farther than 1e15.  A splat at the camera's own position has no
-// direction: the bands contribute nothing.  Forward (v_out NULL): the values of all views at out.  Backward: g receives the
+// direction: the bands contribute nothing, and at degree 0 no position matters, not even one that is not finite.  Forward (v_out NULL): the values of all views at out.  Backward: g receives the
 // gradients of the mean (3), of DC (3) and of the coefficients (45).
 __device__ __noinline__ void eval_checked(const SsbSplats sp, const float* sh, const void* rows, int64_t i, int64_t n, int views,
                                           const float* viewmats, int n_sh, float* out, const float* v_out, float* g) {
@@ -299,6 +305,7 @@ __device__ __noinline__ void eval_checked(const SsbSplats sp, const float* sh, c
                     g[6 + 3 * j + ch] += o.p[j] * sh_constant(j) * go[ch];
                 }
             }
+            if (n_sh == 0) continue;
             sh_polynomials_vjp(dir, o, w, vm);
             for (int k = 0; k < 3; ++k) g[k] += vm[k] * dir.inv;
         }
@@ -627,7 +634,7 @@ __global__ void __launch_bounds__(kProjBlock, kFwdBlocksPerSm) sh_eval_fwd_views
             for (int v = 0; v < v1; ++v, o0 += 3 * n) {
                 Pair d2, c[3];
                 const Directions<Pair> d = view_directions(centres_s[v], mean, d2);
-                least = fminf(least, fminf(d2.x, d2.y)); most = fmaxf(most, fmaxf(d2.x, d2.y));
+                least = fminf(least, fminf(d2.x, d2.y)); most = max_nan(most, d2.x, d2.y);
                 const Pair ny = -1.0f * d.y, c1 = fma_(d.x, d.x, ny * d.y), s1 = (d.x + d.x) * d.y;
                 const Pair c3 = fma_(d.x, c1, ny * s1), s3 = fma_(d.x, s1, d.y * c1);
 #pragma unroll
@@ -758,7 +765,7 @@ __global__ void __launch_bounds__(kProjBlock, kBwdBlocksPerSm) sh_eval_bwd_views
                 slot = (slot + 1) & kGradAhead;
                 const Directions<Pair> d = view_directions(centres_s[v], mean, d2);
                 const Polynomials<Pair> o = sh_polynomials(d);
-                least = fminf(least, fminf(d2.x, d2.y)); most = fmaxf(most, fmaxf(d2.x, d2.y));
+                least = fminf(least, fminf(d2.x, d2.y)); most = max_nan(most, d2.x, d2.y);
 #pragma unroll
                 for (int j = 0; j < kNumSh; ++j) {
                     w[j] = W[3 * j] * g[0];
