@@ -69,8 +69,8 @@ typedef struct SsbSplats {
  * row stands for zeros.  Read by every call that takes an SsbShQuant; written by ssb_quant_encode.  The optimiser does not update
  * it: a trainer keeps fp32 values, encodes them before an iteration's views and applies the gradients to the fp32 values. */
 typedef struct SsbShQuant {
-    void* packed;          /* uint8 [n*45] or uint16 [n*45], or 32-byte rows [n]; NULL = fp32 SH */
-    float* bounds;         /* float2 (min,max) per block of `bounds_stride` cells (not read when bits = 4) */
+    void* packed;          /* uint8 [n*45] or uint16 [n*45] (2-byte aligned), or 32-byte rows [n]; NULL = fp32 SH */
+    float* bounds;         /* float2 (min,max), 8-byte aligned, per block of `bounds_stride` cells (not read when bits = 4) */
     int32_t bits;          /* 4, 8 or 16 (32 / 0 = not quantised) */
     int32_t reserved;
     int64_t bounds_stride; /* cells per bound; 256 for the per-cell-block layout (not read when bits = 4) */

@@ -798,6 +798,8 @@ int check_shq(const SsbSplats* splats, const SsbShQuant* shq, SsbShQuant& out) {
         out = *shq;
         if (out.bounds_stride <= 0) out.bounds_stride = (int64_t)256 * 3 * kNumSh;
         SSB_REQUIRE(out.bounds != nullptr, "quantised SH needs a bounds table");
+        SSB_REQUIRE(((uintptr_t)out.bounds & 7) == 0 && (out.bits == 8 || ((uintptr_t)out.packed & 1) == 0),
+                    "the SH bounds table must start on an 8-byte boundary, 16-bit SH codes on a 2-byte one");
     } else {
         SSB_REQUIRE(splats->features_sh != nullptr, "features_sh is NULL and no quantised SH was given");
     }
