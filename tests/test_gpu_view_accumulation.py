@@ -128,3 +128,60 @@ def test_renders_from_rows_on_several_streams():
         assert torch.equal(image, ref.render(vm[kind], K[kind], kind=kind, sh_bits=4)[0])
         ref.close()
     tr.close()
+
+
+def test_densification_under_dropout_works_on_the_stored_parameters():
+    """Relocation and growth happen between iterations whose views read dropped copies and rows: the parameters stay those of a
+    trainer that keeps its logits itself, unused slots stay unused."""
+    from spirula_studio_b200.densify import DensifyConfig, Densifier
+    cfg, sp, vm, K, gt = scene(n=3000)
+    start = 2000
+    sp["opacities"][:start:17] = -8.0                    # some dead splats among the ones in use
+    host = [torch.from_numpy(np.ascontiguousarray(a)).pin_memory() for a in (vm, K, gt)]
+    tr = Trainer(cfg, sp, device=DEV, view_sh_bits=4, dropout=OPTS)
+    dc = DensifyConfig(refine_start_iter=1, refine_stop_iter=1000, refine_every=3, growth_factor=1.1, noise_lr=0.0)
+    dn = Densifier(tr, dc, start)
+    grown = 0
+    for step in range(8):
+        dn.before_step()
+        before = {k: v.clone() for k, v in tr.params.items()}
+        count = dn.count
+        tr.train_step(*host, 3)
+        drop = dev(O.dropped(0, cfg.n_splats, 1, OPTS.splat_rate, 2 * OPTS.seed, step))
+        assert not tr.grads["means"].view(-1, 3)[drop].any() and not dn.radii[drop].any()      # out of this iteration's views
+        assert not any(g.view(cfg.n_splats, -1)[count:].any() for g in tr.grads.values())      # nor do unused slots appear in them
+        # Adam moves a logit by at most its bias-corrected rate: none has become the logit of a dropped splat, none was compensated
+        # for the rate (0.22 of a logit and more)
+        moved = (tr.params["opacities"] - before["opacities"]).abs()[:count]
+        assert float(moved.max()) <= 3.2 * cfg.lrs["lr_opacities"]
+        stepped = {k: v.clone() for k, v in tr.params.items()}
+        added = dn.after_step(step, 8)
+        grown += added
+        refined = step > dc.refine_start_iter and step % dc.refine_every == 0
+        assert (added > 0) == refined
+        if refined:
+            op = tr.params["opacities"][:dn.count]
+            assert float(op.min()) > -10.0               # relocated and new splats start from stored logits, none from a dropped one
+            assert float((torch.sigmoid(op) <= dc.min_opacity).double().mean()) < 0.01
+        else:
+            assert torch.equal(tr.params["features_sh"], stepped["features_sh"])
+        assert bool((tr.params["opacities"][dn.count:] == -30.0).all())
+    assert grown > 0
+    for k, v in tr.params.items():
+        assert bool(torch.isfinite(v.view(cfg.n_splats, -1)[:dn.count]).all()), k
+    tr.close()
+
+
+def test_splat_dropout_over_sixteen_bit_sh_values():
+    """Opacities are fp32 whatever the SH values are stored in."""
+    cfg, sp, vm, K, gt = scene()
+    cfg.sh_value_bits, cfg.sh_optim_bits = 16, 8
+    opts = DropoutOptions(splat_rate=0.3, seed=5)
+    got = gradients(cfg, sp, vm, K, gt, dropout=opts)
+    op, slope, _ = O.dropout_opacities(sp["opacities"], 0, 0.3, 10, 0)
+    ref = gradients(cfg, {**sp, "opacities": op.astype(np.float32)}, vm, K, gt)
+    ref["opacities"] = ref["opacities"] * dev(slope).float()
+    drop = dev(O.dropped(0, cfg.n_splats, 1, 0.3, 10, 0))
+    for k in got:
+        assert close(got[k], ref[k]), k
+        assert not got[k].view(cfg.n_splats, -1)[drop].any(), k

@@ -253,3 +253,27 @@ def test_options_that_the_library_cannot_take_are_refused_when_they_are_set(fake
     with pytest.raises(ValueError):
         make(fake, dropout=DropoutOptions(**bad))
     make(fake, dropout=DropoutOptions(splat_rate=1.0 - 2.0 ** -24, sh_rate=0.0, sh_group=2 ** 31 - 1))
+
+
+def test_every_rank_draws_the_masks_of_the_whole_array(fake, monkeypatch):
+    """Ranks hold the same parameters and see other views: what their views read must be the same copies."""
+    monkeypatch.setattr(torch.distributed, "all_reduce", lambda *a, **kw: None)
+    drawn = []
+    for rank in range(2):
+        tr = make(fake, dropout=OPTS, world_size=2, rank=rank, grad_sync="nccl")
+        for _ in range(2):
+            fake.calls.clear()
+            views(tr, count=1 + rank)
+            tr.allreduce_grads()
+            tr.optimizer_step(3)
+            for name, args in fake.calls:
+                if "dropout" in name:
+                    d = [a._obj for a in args if isinstance(getattr(a, "_obj", None), L.SsbDropout)][0]
+                    plain = [handle(a) for a in args if not hasattr(a, "_obj")]
+                    sizes = [a for a in plain if a in (0, N, 45 * N, OPTS.sh_group)]
+                    drawn.append((rank, name, d.rate, d.seed, d.offset, tuple(sizes)))
+    mine = [[c[1:] for c in drawn if c[0] == r] for r in range(2)]
+    assert mine[0] == mine[1] and len(mine[0]) == 8
+    assert [c[3] for c in mine[0]] == [0] * 4 + [1] * 4               # the iteration's number
+    assert {(c[1], c[2]) for c in mine[0]} == {(float(np.float32(OPTS.splat_rate)), 2 * OPTS.seed), (float(np.float32(OPTS.sh_rate)), 2 * OPTS.seed + 1)}
+    assert all(0 in c[4] and (N in c[4] or 45 * N in c[4]) for c in mine[0])
