@@ -184,6 +184,7 @@ int ssb_project_bwd(const SsbSplats* splats, const SsbShQuant* shq, int64_t n,
  * src/shaders/harmonics.slang:154-251.  The colour of the projection is max(value + 0.5, 0).
  * Of `splats`, means, features_dc (NULL: zeros) and features_sh (when shq names no codes) are read; of `cams`, d_viewmats,
  * count and sh_degree_plus1.  A splat at the camera's centre has no direction: its value is the features_dc term.
+ * At degree 0 the means do not matter and have no gradient, whatever they hold.
  * ssb_sh_eval_bwd: gradients of means, features_dc and features_sh (the coefficients' values, whatever they are stored in), summed
  * over the views in an order that depends on the sizes only; an array that is NULL in `grads` is not wanted.  accumulate != 0 adds to the arrays.  Coefficients
  * above the active degree get zero. */

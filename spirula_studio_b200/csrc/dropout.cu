@@ -56,7 +56,8 @@ constexpr int kDropTile = kDropThreads * kDropChunks * 4;          // values per
 
 // Every value decides for itself: a thread's four values are the four words of one generator block, so the decisions never
 // leave registers.  Chunks start on multiples of four of the whole array's numbering.  Bound by memory, 8 bytes a value: 135M values in
-// 169 us, 6.4 TB/s, 98 % of the copy bandwidth; the generator's ten rounds fit behind it.
+// 167 us, 6.5 TB/s, 99 % of the copy bandwidth; the generator's ten rounds fit behind it.  Arrays off the numbering's 16-byte
+// boundaries (VEC = false) take four 4-byte accesses per chunk: 45M values 82 us where 16-byte ones take 56.
 // One chunk a thread less or more: 167 (two) and 160 us (eight) where four took 157 on the same day.
 template <bool VEC>
 __global__ void __launch_bounds__(kDropThreads) dropout_values_kernel(const float* x, float* y, int64_t first, int64_t count, DropArgs a) {
@@ -78,8 +79,9 @@ __global__ void __launch_bounds__(kDropThreads) dropout_values_kernel(const floa
 }
 
 // Groups of several values: the decisions of the groups that a block's tile touches are made once, one generator block per
-// four groups, and kept as one byte each in shared memory while the tile's values are on their way.  45M values in groups of three: 56 us,
-// 6.4 TB/s, 98 % of the copy bandwidth; with a 64-bit place per value it was 69 us and bound by integer arithmetic.
+// four groups, and kept as one byte each in shared memory while the tile's values are on their way.  45M values in groups of three: 55 us,
+// 6.5 TB/s, 99 % of the copy bandwidth (75 where the two arrays lie differently in their 16 bytes); with a 64-bit place per value it was
+// 69 us and bound by integer arithmetic.
 struct GroupArgs {
     uint32_t group, magic;
     uint32_t first_rem;        // place of the first value in its group
@@ -138,7 +140,7 @@ struct OpacityArgs {
 
 
 // 1 - e^-d for d > 0 to within 2^-22.  Below 1.375 as d P(d), P the polynomial of degree seven that fits (1 - e^-d) / d there
-// (Chebyshev nodes; 2^-29.8 off, 2.7 half-ulps as evaluated); above it the hardware exponential, whose 2 ulp and the
+// (Chebyshev nodes; with fp32 coefficients 2^-24.9 off, 2.7 half-ulps as evaluated); above it the hardware exponential, whose 2 ulp and the
 // argument's rounding weigh e^-d / (1 - e^-d) <= 0.34 of themselves.  Other d are not used (the opacity is then limited).  expm1f
 // instead made the two calls take 68 instead of 55 us for 10M opacities.
 __device__ __forceinline__ float one_minus_exp_neg(float d) {
@@ -170,8 +172,9 @@ __device__ __forceinline__ float drop_opacity(float x, float v, bool dropped, co
 // hardware logarithm).
 constexpr int kOpacityChunks = 2;
 
-// 8 bytes a splat forward, 12 backward.  10M splats: 20.8 to 22.8 and 24.0 us; ssb_dropout, which moves the forward call's bytes with a third of
-// its arithmetic, takes 16.0 at that size, a device copy of torch's 20.7.
+// 8 bytes a splat forward, 12 backward.  10M splats: 20.8 to 22.9 and 23.7 us (23.0 and 27.1 with VEC = false); ssb_dropout, which moves the
+// forward call's bytes with a third of its arithmetic, takes 16.4 at that size, a device copy of torch's 20.9.  The forward call issues 48
+// instructions a value on 74 % of the cycles.
 
 template <bool BWD, bool VEC>
 __global__ void __launch_bounds__(kDropThreads) dropout_opacity_kernel(const float* x, const float* v, float* out, int64_t first, int64_t count,
@@ -239,7 +242,8 @@ static OpacityArgs opacity_args(float rate) {
     return o;
 }
 
-// Whether value `first` being at p leaves the multiples of four of the numbering on 16-byte boundaries.
+// Whether value `first` being at p leaves the multiples of four of the numbering on 16-byte boundaries: then chunks travel as 16-byte
+// accesses, otherwise as 4-byte ones (the kernels' comments have both times).
 static bool chunk_aligned(const void* p, int64_t first) { return (((uintptr_t)p >> 2) & 3) == (uintptr_t)(first & 3); }
 
 static int launch_opacity(bool bwd, const float* x, const float* v, float* out, int64_t first, int64_t count, const SsbDropout* d, const DropArgs& a,

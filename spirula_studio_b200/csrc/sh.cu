@@ -158,7 +158,8 @@ int launch_sh_rows_decode(const void* d_rows, int64_t n, float* d_values, cudaSt
 // splats at once, 128 apart, with the coefficients in registers, and all its arithmetic is on pairs, one packed single-precision
 // instruction for two results.  What limits that is the register file: a packed multiply-add on three different register pairs was
 // measured at three cycles per scheduler, a scalar one at 1.9, so a pair costs less than two scalars; one splat per thread, scalar or
-// packed over coefficients, took 76 and 81 us where this form takes 64 (1M splats, 16 views, forward) and 157 against 154 backward.
+// packed over coefficients, took 76 and 81 us where this form takes 64 (1M splats, 16 views, forward) and 157 against 153 backward.
+// The active degree is no part of the kernels' types: below degree 3 they do the same work on zeros (degree 0: 60 and 143 us, degrees 1 and 2 as 3).
 typedef float2 Pair;
 __device__ __forceinline__ Pair operator+(Pair a, Pair b) { return __fadd2_rn(a, b); }
 __device__ __forceinline__ Pair operator*(Pair a, Pair b) { return __fmul2_rn(a, b); }
@@ -586,13 +587,13 @@ __device__ __forceinline__ void to_azimuthal(Pair A[16 * 3], const Pair W[kShPer
     }
 }
 
-// What the registers allow (150 and 252 per thread); the grids are this many blocks, which walk the tiles.  Four forward blocks
-// make the compiler spill: 73 us against 64.
+// What the registers allow (156 forward; backward 252 from rows, 255 and 24 bytes of spills from other storages); the grids are this many
+// blocks, which walk the tiles.  Four forward blocks make the compiler spill: 73 us against 64.
 constexpr int kFwdBlocksPerSm = 3, kBwdBlocksPerSm = 2;
 constexpr int kMaxSplit = 8;                   // blocks that share a tile's views in the backward pass, a cluster
 
 // Per (splat, view): the direction (12 operations), the azimuthal functions (7) and 45 multiply-adds.  1M splats, 16 views: 64 us;
-// 20.8M packed instructions at the three cycles of the register file are 55 us, the bytes (248 MB) 38 us.
+// 20.1M packed instructions at the three cycles of the register file are 52 us, the bytes (248 MB) 38 us.
 template <bool ROWS>
 __global__ void __launch_bounds__(kProjBlock, kFwdBlocksPerSm) sh_eval_fwd_views_kernel(SsbSplats sp, SsbShQuant shq, int64_t n, int views,
                                                                                         const float* __restrict__ viewmats, int n_sh,
@@ -711,7 +712,7 @@ __device__ __forceinline__ void join_span(float* dst, float* span_s, int count, 
 
 // Per (splat, view): direction and polynomials (35 operations), 45 multiply-adds for the coefficients' gradients, 45 for the sums w_j
 // and 40 for the mean's.  The 45 gradients of both splats stay in registers over all views, so nothing is added in memory and the sum
-// has one order.  1M splats, 16 views: 154 us; 47.5M packed instructions at three cycles are 125 us, the bytes (440 MB) 67 us.
+// has one order.  1M splats, 16 views: 153 us; 47.1M packed instructions at three cycles are 122 us, the bytes (440 MB) 67 us.
 template <bool ROWS>
 __global__ void __launch_bounds__(kProjBlock, kBwdBlocksPerSm) sh_eval_bwd_views_kernel(SsbSplats sp, SsbShQuant shq, int64_t n, int views,
                                                                                         const float* __restrict__ viewmats, int n_sh,

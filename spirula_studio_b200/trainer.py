@@ -512,7 +512,9 @@ class Trainer:
     def render(self, viewmat, intrin, kind=0, depth=False, sh_bits=None):
         """One image of the current splats, forward only (the viewer's path): viewmat [16] / intrin [4] as numpy or tensors.
         Returns (rgb [H][W][3], transmittance [H][W]) and, with depth=True, the ray-depth image as a third tensor.
-        sh_bits=4 renders from the SH values in 4-bit rows (the default of a trainer whose views read them), 32 from the stored ones."""
+        sh_bits=4 renders from the SH values in 4-bit rows (the default of a trainer whose views read them), 32 from the stored ones.  The
+        rows are encoded anew for every image, which takes longer than reading them saves (1M splats, 1920x1080: 0.685 ms against
+        0.655): sh_bits=4 shows what the rows look like."""
         sh_bits = self.view_sh_bits if sh_bits is None else sh_bits
         if sh_bits not in (4, 32):
             raise ValueError(f"sh_bits must be 4 or 32, not {sh_bits}")
